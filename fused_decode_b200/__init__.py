@@ -15,15 +15,31 @@ from fused_decode_b200.ops import (
     rope,
     swiglu,
 )
+from fused_decode_b200.ops_fp8 import (
+    add_rms_norm_fp8,
+    linear_act,
+    linear_fp8,
+    post_attn_mlp_fp8,
+    quantize_fp8,
+    rms_norm_fp8,
+    swiglu_fp8,
+)
 
 __all__ = [
     "DECODE_LINEAR_MAX_M",
     "add_rms_norm",
+    "add_rms_norm_fp8",
+    "linear_act",
     "linear_decode",
+    "linear_fp8",
     "post_attn_mlp",
+    "post_attn_mlp_fp8",
+    "quantize_fp8",
     "rms_norm",
+    "rms_norm_fp8",
     "rope",
     "swiglu",
+    "swiglu_fp8",
 ]
 __version__ = "0.1.0"
 

@@ -19,9 +19,11 @@ LIB_NAME = "libfd_b200.so"
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), LIB_NAME)
 
 # fd_dtype
-FD_F16, FD_BF16, FD_F32 = 0, 1, 2
+FD_F16, FD_BF16, FD_F32, FD_E4M3 = 0, 1, 2, 3
 # fd_kind
 FD_KIND_DOT, FD_KIND_SIMT = 0, 1
+# fd_act
+ACTIVATIONS = {None: 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4}
 
 _DTYPE_CODE = {torch.float16: FD_F16, torch.bfloat16: FD_BF16, torch.float32: FD_F32}
 
@@ -153,6 +155,42 @@ SIGNATURES: dict[str, tuple] = {
             c_vp, c_size, c_vp,          # workspace, bytes, stream
         ],
     ),
+    "fd_quantize_fp8_out": (c_i32, [_P_ROWS, _P_ROWS, c_vp, c_vp]),
+    "fd_rms_fp8_out": (c_i32, [_P_ROWS, _P_ROWS, c_vp, c_i32, c_i64, _P_ROWS, c_vp, _P_ROWS, c_f32, c_vp]),
+    "fd_swiglu_fp8_out": (c_i32, [_P_ROWS, _P_ROWS, _P_ROWS, c_vp, c_vp]),
+    "fd_linear_act_out": (
+        c_i32,
+        [
+            c_vp, c_i64, c_i64,          # x, sxm, sxk
+            c_vp, c_i64, c_i64,          # w, swn, swk
+            c_vp, c_i32, c_i64,          # bias, bias_dtype, sbias
+            c_vp, c_i32, c_i64, c_i64,   # row_add, ra_dtype, srm, srn
+            c_vp, c_i64, c_i64,          # y, sym, syn
+            c_i32, c_i32, c_i64, c_i64, c_i64, c_vp,  # dtype, act, m, n, k, stream
+        ],
+    ),
+    "fd_linear_fp8_out": (
+        c_i32,
+        [
+            c_vp, c_i64, c_i64, c_vp,    # x, sxm, sxk, x_scale
+            c_vp, c_i64, c_i64, c_vp,    # w, swn, swk, w_scale
+            c_vp, c_i32, c_i64,          # bias, bias_dtype, sbias
+            c_vp, c_i32, c_i64, c_i64,   # row_add, ra_dtype, srm, srn
+            c_vp, c_i64, c_i64,          # y, sym, syn
+            c_i32, c_i32, c_i64, c_i64, c_i64, c_vp,  # out_dtype, act, m, n, k, stream
+        ],
+    ),
+    "fd_post_attn_mlp_fp8_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
+    "fd_post_attn_mlp_fp8_out": (
+        c_i32,
+        [
+            c_vp, c_i64, c_vp, c_i32, c_i64,   # hidden, s_hidden, norm_w, norm_dtype, s_norm
+            c_vp, c_i64, c_vp,                 # w_gate_up, s_gu, gate_up_scale
+            c_vp, c_i64, c_vp,                 # w_down, s_down, down_scale
+            c_vp, c_i32, c_i64, c_i64, c_i64,  # out, dtype, m, h, i
+            c_f32, c_vp, c_size, c_vp,         # eps, workspace, bytes, stream
+        ],
+    ),
     "fd_residual_add_out": (c_i32, [c_vp, c_vp, c_vp, c_i32, c_i64, c_vp]),
     "fd_copy": (c_i32, [c_vp, c_vp, c_size, c_vp]),
     "fd_triad": (c_i32, [c_vp, c_vp, c_vp, c_i64, c_i32, c_f32, c_vp]),
@@ -244,7 +282,7 @@ def rows(layout) -> FdRows:
     t = layout.tensor
     return FdRows(
         t.data_ptr(),
-        dtype_code(t.dtype),
+        FD_E4M3 if t.dtype == torch.float8_e4m3fn else dtype_code(t.dtype),
         0,
         layout.a,
         layout.b,

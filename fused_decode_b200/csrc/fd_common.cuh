@@ -211,7 +211,7 @@ namespace fd_host {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-inline int elem_size(int dtype) { return dtype == FD_F32 ? 4 : 2; }
+inline int elem_size(int dtype) { return dtype == FD_F32 ? 4 : dtype == FD_E4M3 ? 1 : 2; }
 
 inline bool valid_dtype(int dtype) { return dtype == FD_F16 || dtype == FD_BF16 || dtype == FD_F32; }
 

@@ -477,6 +477,190 @@ def residual_add_out(partial: torch.Tensor, residual: torch.Tensor, out: torch.T
     _capi.check(status, "fd_residual_add_out")
 
 
+# ------------------------------------------------------------------ 8-bit rows
+def _scale_rows(scale: torch.Tensor, layout: RowLayout) -> None:
+    if scale.dtype != torch.float32 or not scale.is_contiguous() or scale.numel() != layout.rows:
+        raise ValueError("scale must be a contiguous float32 tensor with one element per row")
+
+
+def quantize_fp8_out(x: torch.Tensor, out: torch.Tensor, scale: torch.Tensor) -> None:
+    """Rows of ``x`` to e4m3 values in ``out`` with one fp32 ``scale`` each."""
+    lx, lq = row_layout(x), row_layout(out)
+    _same_grid(lx, lq, "out")
+    _scale_rows(scale, lx)
+    if lx.rows == 0:
+        return
+    lib = _capi.load()
+    with torch.cuda.device(x.device):
+        status = lib.fd_quantize_fp8_out(_capi.rows(lx), _capi.rows(lq), scale.data_ptr(), _capi.stream_of(x))
+    _capi.check(status, "fd_quantize_fp8_out")
+    _write_back(lq, out)
+
+
+def rms_fp8_out(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float,
+    out: torch.Tensor,
+    scale: torch.Tensor,
+    residual: torch.Tensor | None = None,
+    residual_out: torch.Tensor | None = None,
+) -> None:
+    """RMSNorm / fused add+RMSNorm with the normalised rows in e4m3 (``out``, ``scale``)."""
+    lx, lq = row_layout(x), row_layout(out)
+    _same_grid(lx, lq, "out")
+    _scale_rows(scale, lx)
+    lr = row_layout(residual) if residual is not None else None
+    lro = row_layout(residual_out) if residual_out is not None else None
+    if lr is not None:
+        _same_grid(lx, lr, "residual")
+    if lro is not None:
+        _same_grid(lx, lro, "residual_out")
+    if lx.rows == 0:
+        return
+    lib = _capi.load()
+    with torch.cuda.device(x.device):
+        status = lib.fd_rms_fp8_out(
+            _capi.rows(lx), _capi.rows(lr) if lr is not None else None,
+            weight.data_ptr(), _capi.dtype_code(weight.dtype), int(weight.stride(0)),
+            _capi.rows(lq), scale.data_ptr(), _capi.rows(lro) if lro is not None else None,
+            float(eps), _capi.stream_of(x),
+        )
+    _capi.check(status, "fd_rms_fp8_out")
+    _write_back(lq, out)
+    if lro is not None:
+        _write_back(lro, residual_out)
+
+
+def swiglu_fp8_out(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor, scale: torch.Tensor) -> None:
+    """``silu(gate) * up`` in e4m3 (``out``, ``scale``)."""
+    lg, lu, lq = row_layout(gate), row_layout(up), row_layout(out)
+    _same_grid(lg, lu, "up")
+    _same_grid(lg, lq, "out")
+    _scale_rows(scale, lg)
+    if lg.rows == 0:
+        return
+    lib = _capi.load()
+    with torch.cuda.device(gate.device):
+        status = lib.fd_swiglu_fp8_out(_capi.rows(lg), _capi.rows(lu), _capi.rows(lq), scale.data_ptr(),
+                                       _capi.stream_of(gate))
+    _capi.check(status, "fd_swiglu_fp8_out")
+    _write_back(lq, out)
+
+
+# ------------------------------------------------------------------ products
+def _epilogue_args(bias: torch.Tensor | None, row_add: torch.Tensor | None) -> tuple:
+    """(bias, dtype, stride, row_add, dtype, row stride, column stride) of the C ABI."""
+    b = (None, 0, 0) if bias is None else (bias.data_ptr(), _capi.dtype_code(bias.dtype), int(bias.stride(0)))
+    if row_add is None:
+        return (*b, None, 0, 0, 0)
+    srm = 0 if row_add.shape[0] == 1 else int(row_add.stride(0))
+    srn = 0 if row_add.shape[1] == 1 else int(row_add.stride(1))
+    return (*b, row_add.data_ptr(), _capi.dtype_code(row_add.dtype), srm, srn)
+
+
+def linear_act_out(
+    x: torch.Tensor,
+    weight: torch.Tensor,
+    y: torch.Tensor,
+    *,
+    bias: torch.Tensor | None = None,
+    activation: str | None = None,
+    row_add: torch.Tensor | None = None,
+) -> None:
+    """``y = act(x @ weight.T [+ bias]) [+ row_add]`` for ``x`` [M, K], any M.
+
+    ``row_add`` is 2-D with each dim 1 or full, as in ``linear_out``; ``y``
+    may be ``row_add`` itself.
+    """
+    m, k = x.shape
+    n = weight.shape[0]
+    if weight.shape[1] != k:
+        raise ValueError(f"K mismatch: x has {k}, weight has {weight.shape[1]}")
+    if y.shape != (m, n):
+        raise ValueError(f"y shape {tuple(y.shape)} != {(m, n)}")
+    if m == 0 or n == 0:
+        return
+    lib = _capi.load()
+    with torch.cuda.device(x.device):
+        status = lib.fd_linear_act_out(
+            x.data_ptr(), int(x.stride(0)), int(x.stride(1)),
+            weight.data_ptr(), int(weight.stride(0)), int(weight.stride(1)),
+            *_epilogue_args(bias, row_add),
+            y.data_ptr(), int(y.stride(0)), int(y.stride(1)),
+            _capi.dtype_code(x.dtype), _capi.ACTIVATIONS[activation], m, n, k, _capi.stream_of(x),
+        )
+    _capi.check(status, "fd_linear_act_out")
+
+
+def linear_fp8_out(
+    x: torch.Tensor,
+    x_scale: torch.Tensor,
+    weight: torch.Tensor,
+    weight_scale: torch.Tensor,
+    y: torch.Tensor,
+    *,
+    bias: torch.Tensor | None = None,
+    activation: str | None = None,
+    row_add: torch.Tensor | None = None,
+) -> None:
+    """``linear_act_out`` for e4m3 ``x`` [M, K] and ``weight`` [N, K] with
+    contiguous fp32 scales of one element per row."""
+    m, k = x.shape
+    n = weight.shape[0]
+    if weight.shape[1] != k:
+        raise ValueError(f"K mismatch: x has {k}, weight has {weight.shape[1]}")
+    if y.shape != (m, n):
+        raise ValueError(f"y shape {tuple(y.shape)} != {(m, n)}")
+    for name, s, rows in (("x_scale", x_scale, m), ("weight_scale", weight_scale, n)):
+        if s.dtype != torch.float32 or not s.is_contiguous() or s.numel() != rows:
+            raise ValueError(f"{name} must be a contiguous float32 tensor of {rows} elements")
+    if m == 0 or n == 0:
+        return
+    lib = _capi.load()
+    with torch.cuda.device(x.device):
+        status = lib.fd_linear_fp8_out(
+            x.data_ptr(), int(x.stride(0)), int(x.stride(1)), x_scale.data_ptr(),
+            weight.data_ptr(), int(weight.stride(0)), int(weight.stride(1)), weight_scale.data_ptr(),
+            *_epilogue_args(bias, row_add),
+            y.data_ptr(), int(y.stride(0)), int(y.stride(1)),
+            _capi.dtype_code(y.dtype), _capi.ACTIVATIONS[activation], m, n, k, _capi.stream_of(x),
+        )
+    _capi.check(status, "fd_linear_fp8_out")
+
+
+def post_attn_mlp_fp8_out(
+    hidden2: torch.Tensor,
+    norm_weight: torch.Tensor,
+    w_gate_up: torch.Tensor,
+    gate_up_scale: torch.Tensor,
+    w_down: torch.Tensor,
+    down_scale: torch.Tensor,
+    out2: torch.Tensor,
+    eps: float,
+) -> None:
+    """RMSNorm -> 8-bit gate/up product -> SwiGLU -> 8-bit down product (+ hidden) into ``out2``.
+
+    ``hidden2`` [M, H] and the e4m3 weights have unit stride along their last
+    dimension; ``out2`` is contiguous.  The intermediates live in a buffer of
+    the caching allocator, so concurrent streams and captured graphs share none.
+    """
+    m, h = hidden2.shape
+    i = w_down.shape[1]
+    lib = _capi.load()
+    ws = torch.empty(lib.fd_post_attn_mlp_fp8_workspace_bytes(m, h, i), dtype=torch.uint8, device=hidden2.device)
+    with torch.cuda.device(hidden2.device):
+        status = lib.fd_post_attn_mlp_fp8_out(
+            hidden2.data_ptr(), int(hidden2.stride(0)),
+            norm_weight.data_ptr(), _capi.dtype_code(norm_weight.dtype), int(norm_weight.stride(0)),
+            w_gate_up.data_ptr(), int(w_gate_up.stride(0)), gate_up_scale.data_ptr(),
+            w_down.data_ptr(), int(w_down.stride(0)), down_scale.data_ptr(),
+            out2.data_ptr(), _capi.dtype_code(hidden2.dtype), m, h, i, float(eps),
+            ws.data_ptr(), ws.numel(), _capi.stream_of(hidden2),
+        )
+    _capi.check(status, "fd_post_attn_mlp_fp8_out")
+
+
 # ------------------------------------------------------------------ roofs
 def launch_copy(dst: torch.Tensor, src: torch.Tensor) -> None:
     """``dst[:] = src`` with the 16-byte streaming copy (reference kernels.py:849-852)."""

@@ -30,7 +30,8 @@ extern "C" {
 typedef enum {
   FD_F16 = 0,
   FD_BF16 = 1,
-  FD_F32 = 2
+  FD_F32 = 2,
+  FD_E4M3 = 3 /* 8-bit values: only where an entry point names it */
 } fd_dtype;
 
 typedef enum {
@@ -47,6 +48,15 @@ typedef enum {
   FD_KIND_DOT = 0,  /* tensor-core path (reference "dot") */
   FD_KIND_SIMT = 1  /* CUDA-core fp32 FMA path (reference "simt") */
 } fd_kind;
+
+/* Activations of the matrix products' epilogue. */
+typedef enum {
+  FD_ACT_NONE = 0,
+  FD_ACT_RELU = 1,
+  FD_ACT_SILU = 2,      /* v * sigmoid(v) */
+  FD_ACT_GELU = 3,      /* 0.5 v (1 + erf(v / sqrt(2))) */
+  FD_ACT_GELU_TANH = 4  /* 0.5 v (1 + tanh(sqrt(2/pi) (v + 0.044715 v^3))) */
+} fd_act;
 
 /* A batch of rows of length n.  Row r = (ia, ib, ic) with r = (ia*b + ib)*c + ic
  * starts at ptr + ia*sa + ib*sb + ic*sc; element j of the row is at +j*col.
@@ -284,6 +294,66 @@ int fd_mlp_gate_up_out(const void* hidden, const void* norm_w, int32_t norm_dtyp
                        const void* w_gate_up, int64_t s_gu, void* mid, int32_t dtype,
                        int32_t m, int64_t h, int64_t i, float eps, int32_t kind,
                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- 8-bit rows and products (no counterpart in the reference, whose
+ * operators are 16-bit; they stand beside its rms_norm, add_rms_norm, swiglu,
+ * linear_decode and post_attn_mlp, ops.py:72-315).
+ *
+ * Rows to 8 bits: `out` is an fd_rows grid of FD_E4M3 values on the input's
+ * grid, `scale` one contiguous fp32 per row in row order:
+ *   a = max(max_j |y_j|, 2^-64), scale = a / 448, out_j = e4m3(y_j * (448 / a))
+ * (to nearest even, saturating; a NaN in y makes the row's scale NaN), where
+ * the fp32 row y is
+ *   fd_quantize_fp8_out: x
+ *   fd_rms_fp8_out:      s * rsqrt(mean(s*s) + eps) * weight, s = x (+ residual)
+ *                        residual_out = round(s) when a residual is given
+ *                        (both or neither; it may be the residual itself)
+ *   fd_swiglu_fp8_out:   silu(gate) * up
+ * Inputs are f16 or bf16 with any strides. */
+int fd_quantize_fp8_out(const fd_rows* x, const fd_rows* out, float* scale, void* stream);
+int fd_rms_fp8_out(const fd_rows* x, const fd_rows* residual, const void* weight,
+                   int32_t w_dtype, int64_t w_stride, const fd_rows* out, float* scale,
+                   const fd_rows* residual_out, float eps, void* stream);
+int fd_swiglu_fp8_out(const fd_rows* gate, const fd_rows* up, const fd_rows* out,
+                      float* scale, void* stream);
+
+/* y[m, n] = round(act(sum_k x[m, k] * w[n, k] + bias[n]) + row_add[m, n]) for
+ * any m, fp32 sums.  x, w and y share dtype (f16 or bf16); act is an fd_act;
+ * bias and row_add are f16, bf16 or f32 and may be NULL (stride 0 where
+ * row_add broadcasts; y may be row_add itself).  No workspace. */
+int fd_linear_act_out(const void* x, int64_t sxm, int64_t sxk,
+                      const void* w, int64_t swn, int64_t swk,
+                      const void* bias, int32_t bias_dtype, int64_t sbias,
+                      const void* row_add, int32_t ra_dtype, int64_t srm, int64_t srn,
+                      void* y, int64_t sym, int64_t syn,
+                      int32_t dtype, int32_t act, int64_t m, int64_t n, int64_t k, void* stream);
+
+/* The same product of e4m3 operands with scales:
+ * y[m, n] = round(act(sum_k x[m, k] * w[n, k] * x_scale[m] * w_scale[n] + bias[n]) + row_add[m, n]),
+ * x_scale [m] and w_scale [n] contiguous fp32, y f16 or bf16 (out_dtype). */
+int fd_linear_fp8_out(const void* x, int64_t sxm, int64_t sxk, const float* x_scale,
+                      const void* w, int64_t swn, int64_t swk, const float* w_scale,
+                      const void* bias, int32_t bias_dtype, int64_t sbias,
+                      const void* row_add, int32_t ra_dtype, int64_t srm, int64_t srn,
+                      void* y, int64_t sym, int64_t syn,
+                      int32_t out_dtype, int32_t act, int64_t m, int64_t n, int64_t k, void* stream);
+
+/* post_attn_mlp with 8-bit weights and activations, any number of rows:
+ *   q, s    = rms_fp8(hidden, norm_w)
+ *   gate_up = round(linear_fp8(q, s, w_gate_up))      (w_gate_up e4m3 [2i, h])
+ *   p, t    = swiglu_fp8(gate, up)
+ *   out     = round(linear_fp8(p, t, w_down) + hidden)  (w_down e4m3 [h, i])
+ * hidden rows are s_hidden apart, the weights' rows s_gu and s_down (unit
+ * stride along k); out [m, h] is contiguous and may not overlap hidden.  The
+ * workspace holds the intermediates (16-byte aligned, any contents); launches
+ * that share one must not overlap in time. */
+size_t fd_post_attn_mlp_fp8_workspace_bytes(int64_t m, int64_t h, int64_t i);
+int fd_post_attn_mlp_fp8_out(const void* hidden, int64_t s_hidden, const void* norm_w,
+                             int32_t norm_dtype, int64_t s_norm,
+                             const void* w_gate_up, int64_t s_gu, const float* gate_up_scale,
+                             const void* w_down, int64_t s_down, const float* down_scale,
+                             void* out, int32_t dtype, int64_t m, int64_t h, int64_t i,
+                             float eps, void* workspace, size_t workspace_bytes, void* stream);
 
 /* out[j] = round(partial[j] + residual[j]) for n contiguous elements: the
  * residual add after a tensor-parallel allreduce of fp32 partials (the
