@@ -180,6 +180,8 @@ SIGNATURES: dict[str, tuple] = {
             c_i32, c_i32, c_i64, c_i64, c_i64, c_vp,  # out_dtype, act, m, n, k, stream
         ],
     ),
+    "fd_product_status": (c_i32, [ctypes.POINTER(c_i32), c_vp]),
+    "fd_product_reset": (c_i32, [c_vp]),
     "fd_post_attn_mlp_fp8_workspace_bytes": (c_size, [c_i64, c_i64, c_i64]),
     "fd_post_attn_mlp_fp8_out": (
         c_i32,

@@ -629,6 +629,18 @@ def linear_fp8_out(
     _capi.check(status, "fd_linear_fp8_out")
 
 
+def product_status(device: torch.device | None = None) -> int:
+    """Non-zero once a bounded wait inside a product kernel expired on
+    ``device`` (that call's output is not valid); waits for its current stream."""
+    import ctypes
+
+    word = ctypes.c_int32()
+    with torch.cuda.device(device):
+        status = _capi.load().fd_product_status(word, torch.cuda.current_stream().cuda_stream)
+    _capi.check(status, "fd_product_status")
+    return word.value
+
+
 def post_attn_mlp_fp8_out(
     hidden2: torch.Tensor,
     norm_weight: torch.Tensor,

@@ -338,6 +338,15 @@ int fd_linear_fp8_out(const void* x, int64_t sxm, int64_t sxk, const float* x_sc
                       void* y, int64_t sym, int64_t syn,
                       int32_t out_dtype, int32_t act, int64_t m, int64_t n, int64_t k, void* stream);
 
+/* Health of the two products above on the current device (no workspace, so
+ * the word is the library's own): non-zero once a bounded in-kernel wait of
+ * theirs expired, which makes that call's output invalid.
+ *   fd_product_status: the word after all work enqueued on `stream` so far;
+ *     waits for `stream` to finish.
+ *   fd_product_reset: zero it on `stream`. */
+int fd_product_status(int32_t* status, void* stream);
+int fd_product_reset(void* stream);
+
 /* post_attn_mlp with 8-bit weights and activations, any number of rows:
  *   q, s    = rms_fp8(hidden, norm_w)
  *   gate_up = round(linear_fp8(q, s, w_gate_up))      (w_gate_up e4m3 [2i, h])

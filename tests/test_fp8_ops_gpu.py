@@ -419,6 +419,12 @@ def test_streams_and_graphs():
             assert torch.equal(out, ref)
 
 
+def test_no_wait_expired():
+    from fused_decode_b200 import kernels as K
+
+    assert K.product_status() == 0
+
+
 def test_cuda_refusals():
     """What the checks let through on any device and refuse on a GPU."""
     x = torch.zeros(2, 16, device="cuda", dtype=BF)
