@@ -116,8 +116,212 @@ __global__ void __launch_bounds__(kGenThreads) quant_generic_kernel(QuantArgs a)
   if (threadIdx.x == 0) a.scale[row] = amax / kMax8;
 }
 
+// ============================================================== vectors of 8
+// Rows of 16-byte vectors, each handled by `wpr` warps: every thread keeps VPT
+// vectors of the row in registers, so the inputs are read from HBM once.  The
+// norm needs the sum of squares before any y is known; since
+// max|s * inv * w| = inv * max|s * w|, both reductions run over the row
+// together, at the price of one more pass over the registers for a row whose
+// s * w is not finite.  Bound by HBM for many rows, by one round trip to memory
+// and the reduction for few.
+struct QuantVecArgs {
+  QuantArgs g;
+  int32_t wpr;  // warps per row
+  int32_t rpc;  // rows per CTA
+  int32_t nv;   // vectors per row
+};
+
+struct RowStats {
+  float sum;
+  uint32_t top;
+};
+
+// Sum and maximum over the warps of a row's group; every warp of the CTA takes part.
+FD_DEV RowStats group_reduce(RowStats s, int wpr, int group, float* red_sum, uint32_t* red_top) {
+  s.sum = warp_sum(s.sum);
+  s.top = __reduce_max_sync(0xffffffffu, s.top);
+  if (wpr > 1) {
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) {
+      red_sum[warp] = s.sum;
+      red_top[warp] = s.top;
+    }
+    __syncthreads();
+    s = {0.f, 0u};
+    for (int w = 0; w < wpr; ++w) {
+      s.sum += red_sum[group * wpr + w];
+      s.top = max(s.top, red_top[group * wpr + w]);
+    }
+  }
+  return s;
+}
+
+FD_DEV uint2 pack8_e4m3(const float* f) {
+  auto two = [](float a, float b) -> uint32_t {
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  };
+  return make_uint2(two(f[0], f[1]) | two(f[2], f[3]) << 16, two(f[4], f[5]) | two(f[6], f[7]) << 16);
+}
+
+template <typename T, int OP, int VPT, bool FLAT>
+__global__ void __launch_bounds__(512) quant_vec_kernel(QuantVecArgs a) {
+  __shared__ float red_sum[2][16];
+  __shared__ uint32_t red_top[2][16];
+  constexpr bool kNorm = OP == ROW_RMS || OP == ROW_ADD_RMS;
+  constexpr bool kTwo = OP == ROW_ADD_RMS || OP == ROW_SWIGLU;
+  const int group_threads = 32 * a.wpr;
+  const int group = threadIdx.x / group_threads;
+  const int t = threadIdx.x - group * group_threads;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * a.rpc + group;
+  const bool live = row < a.g.rows;
+  const RowIdx ri = split_row<FLAT>(live ? row : 0, a.g.B, a.g.C);
+  const int wes = a.g.w_dtype == FD_F32 ? 4 : 2;
+  auto weight = [&](int j, float* w) {
+    load8_as_f32(static_cast<const char*>(a.g.w) + static_cast<int64_t>(8 * j) * wes, a.g.w_dtype, w);
+  };
+  grid_dep_wait();
+  grid_dep_launch();
+
+  float s[VPT][8];
+  RowStats st{0.f, 0u};
+  if (live) {
+    const T* xr = reinterpret_cast<const T*>(a.g.x.ptr) + offset_of(a.g.x, ri);
+    const T* rr = kTwo ? reinterpret_cast<const T*>(a.g.r.ptr) + offset_of(a.g.r, ri) : nullptr;
+    uint4 xv[VPT], rv[VPT];
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = t + i * group_threads;
+      if (j < a.nv) {
+        xv[i] = ld_plain16(xr + 8 * j);
+        if (kTwo) rv[i] = ld_plain16(rr + 8 * j);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = t + i * group_threads;
+      if (j < a.nv) {
+        unpack8<T>(xv[i], s[i]);
+        if (kTwo) {
+          float f[8];
+          unpack8<T>(rv[i], f);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) s[i][e] = OP == ROW_SWIGLU ? silu_mul(s[i][e], f[e]) : s[i][e] + f[e];
+        }
+        if (kNorm) {
+          float w[8];
+          weight(j, w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            st.sum += s[i][e] * s[i][e];
+            st.top = max(st.top, abs_bits(s[i][e] * w[e]));
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) st.top = max(st.top, abs_bits(s[i][e]));
+        }
+      }
+    }
+    if (OP == ROW_ADD_RMS) {
+      T* ror = reinterpret_cast<T*>(a.g.ro.ptr) + offset_of(a.g.ro, ri);
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int j = t + i * group_threads;
+        if (j < a.nv) st_stream16(ror + 8 * j, pack8<T>(s[i]));
+      }
+    }
+  }
+  st = group_reduce(st, a.wpr, group, red_sum[0], red_top[0]);
+  float inv = 1.f, amax = __uint_as_float(st.top);
+  if (kNorm) {
+    inv = rsqrtf(st.sum / static_cast<float>(a.g.n) + a.g.eps);
+    if (st.top < 0x7f800000u) {
+      amax *= inv;
+    } else {
+      // s * w overflowed, or holds an infinity or a NaN: the maximum of the
+      // products themselves, as the definition orders them.  With one warp a
+      // row the condition may differ between a CTA's rows, and the reduction
+      // stays within the warp; with more there is one row to a CTA.
+      RowStats again{0.f, 0u};
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int j = t + i * group_threads;
+        if (live && j < a.nv) {
+          float w[8];
+          weight(j, w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) again.top = max(again.top, abs_bits(s[i][e] * inv * w[e]));
+        }
+      }
+      amax = __uint_as_float(group_reduce(again, a.wpr, group, red_sum[1], red_top[1]).top);
+    }
+  }
+  if (!live) return;
+  amax = floor_amax(amax);
+  const float up = kMax8 / amax;
+  uint8_t* qr = reinterpret_cast<uint8_t*>(a.g.q.ptr) + offset_of(a.g.q, ri);
+#pragma unroll
+  for (int i = 0; i < VPT; ++i) {
+    const int j = t + i * group_threads;
+    if (j < a.nv) {
+      float o[8];
+      if (kNorm) {
+        float w[8];
+        weight(j, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = s[i][e] * inv * w[e] * up;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = s[i][e] * up;
+      }
+      *reinterpret_cast<uint2*>(qr + 8 * j) = pack8_e4m3(o);
+    }
+  }
+  if (t == 0) a.g.scale[row] = amax / kMax8;
+}
+
 // ============================================================== host side
 int from_cuda(cudaError_t e) { return e == cudaSuccess ? FD_OK : FD_ERR_LAUNCH; }
+
+// e4m3 rows that can be written 8 values at a time.
+bool rows_vec8(const fd_rows* q) {
+  if (q->col != 1 || reinterpret_cast<uintptr_t>(q->ptr) % 8) return false;
+  return !((q->a > 1 && q->sa % 8) || (q->b > 1 && q->sb % 8) || (q->c > 1 && q->sc % 8));
+}
+
+template <typename T, int OP, int VPT>
+cudaError_t launch_vec2(const QuantVecArgs& a, bool flat, cudaStream_t st) {
+  const dim3 threads(32 * a.wpr * a.rpc);
+  const dim3 blocks(static_cast<unsigned>((a.g.rows + a.rpc - 1) / a.rpc));
+  return flat ? fd_host::launch_pdl(quant_vec_kernel<T, OP, VPT, true>, blocks, threads, 0, st, a)
+              : fd_host::launch_pdl(quant_vec_kernel<T, OP, VPT, false>, blocks, threads, 0, st, a);
+}
+
+// Vectors per thread and warps per row, nv <= 4096.
+template <typename T, int OP>
+cudaError_t launch_vec(QuantVecArgs a, bool flat, cudaStream_t st) {
+  const int nv = a.nv;
+  a.wpr = 1;
+  a.rpc = 4;
+  if (nv <= 32) return launch_vec2<T, OP, 1>(a, flat, st);
+  if (nv <= 64) return launch_vec2<T, OP, 2>(a, flat, st);
+  a.rpc = 1;
+  auto warps = [&](int vpt) { return (nv + 32 * vpt - 1) / (32 * vpt); };
+  // few rows: as many threads a row as a CTA has, for the shortest chain
+  if (a.g.rows <= fd_host::sm_count() && warps(1) <= 16) {
+    a.wpr = warps(1);
+    return launch_vec2<T, OP, 1>(a, flat, st);
+  }
+  if (a.g.rows <= fd_host::sm_count() && warps(2) <= 16) {
+    a.wpr = warps(2);
+    return launch_vec2<T, OP, 2>(a, flat, st);
+  }
+  if (warps(4) <= 16) {
+    a.wpr = warps(4);
+    return launch_vec2<T, OP, 4>(a, flat, st);
+  }
+  a.wpr = warps(8);
+  return launch_vec2<T, OP, 8>(a, flat, st);
+}
 
 template <int OP>
 int launch_quant(const fd_rows* x, const fd_rows* r, const fd_rows* q, const fd_rows* ro, float* scale, const void* w,
@@ -146,6 +350,15 @@ int launch_quant(const fd_rows* x, const fd_rows* r, const fd_rows* q, const fd_
   a.w_stride = w_stride;
   a.eps = eps;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool norm = OP == ROW_RMS || OP == ROW_ADD_RMS;
+  if (x->n > 0 && x->n % 8 == 0 && x->n <= 32768 && rows_vec16(x) && rows_vec8(q) &&
+      (OP == ROW_PLAIN || OP == ROW_RMS || rows_vec16(r)) && (OP != ROW_ADD_RMS || rows_vec16(ro)) &&
+      (!norm || (w_stride == 1 && aligned16(w)))) {
+    const QuantVecArgs v{a, 1, 1, static_cast<int32_t>(x->n / 8)};
+    const bool flat = x->a == 1 && x->b == 1;
+    return from_cuda(x->dtype == FD_BF16 ? launch_vec<__nv_bfloat16, OP>(v, flat, st)
+                                         : launch_vec<__half, OP>(v, flat, st));
+  }
   const dim3 blocks(static_cast<unsigned>(rows));
   return from_cuda(x->dtype == FD_BF16
                        ? launch_pdl(quant_generic_kernel<__nv_bfloat16, OP>, blocks, kGenThreads, 0, st, a)
