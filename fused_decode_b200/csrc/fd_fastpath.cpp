@@ -422,6 +422,232 @@ py::object post_attn_mlp(py::handle hh, py::handle hnw, py::handle hgu, py::hand
   return py::cast(out);
 }
 
+// ------------------------------------------------------------ 8-bit rows
+// ops_fp8.py's outputs: given ones must be what the kernels can write in
+// place, absent ones are fresh.
+bool rows8_for(py::handle hout, py::handle hscale, const at::Tensor& x, at::Tensor* q, at::Tensor* scale, fd_rows* rq) {
+  if (hout.is_none()) {
+    *q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  } else {
+    const at::Tensor* o = as_tensor(hout);
+    if (!o || o->sizes() != x.sizes() || o->scalar_type() != at::kFloat8_e4m3fn || o->device() != x.device())
+      return false;
+    *q = *o;
+  }
+  if (!rows_of(*q, rq)) return false;
+  rq->dtype = FD_E4M3;
+  const c10::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
+  if (hscale.is_none()) {
+    *scale = at::empty(lead, x.options().dtype(at::kFloat));
+  } else {
+    const at::Tensor* o = as_tensor(hscale);
+    if (!o || o->sizes() != lead || o->scalar_type() != at::kFloat || o->device() != x.device() || !o->is_contiguous())
+      return false;
+    *scale = *o;
+  }
+  return true;
+}
+
+py::object quantize_fp8(py::handle hx, py::handle hout, py::handle hscale) {
+  const at::Tensor* x = as_tensor(hx);
+  fd_rows rx, rq;
+  if (!x || !activation(*x) || !rows_of(*x, &rx)) return py::none();
+  const c10::cuda::CUDAGuard guard(x->device());
+  at::Tensor q, scale;
+  if (!rows8_for(hout, hscale, *x, &q, &scale, &rq)) return py::none();
+  if (row_count(rx) > 0)
+    check(fd_quantize_fp8_out(&rx, &rq, scale.data_ptr<float>(), stream_of(*x)), "fd_quantize_fp8_out");
+  return py::make_tuple(q, scale);
+}
+
+py::object rms_norm_fp8(py::handle hx, py::handle hw, py::handle heps, py::handle hout, py::handle hscale) {
+  const at::Tensor* x = as_tensor(hx);
+  const at::Tensor* w = as_tensor(hw);
+  double eps;
+  fd_rows rx, rq;
+  if (!x || !w || !activation(*x) || !norm_weight_ok(*w, *x) || !eps_ok(heps, &eps) || !rows_of(*x, &rx))
+    return py::none();
+  const c10::cuda::CUDAGuard guard(x->device());
+  at::Tensor q, scale;
+  if (!rows8_for(hout, hscale, *x, &q, &scale, &rq)) return py::none();
+  if (row_count(rx) > 0)
+    check(fd_rms_fp8_out(&rx, nullptr, w->data_ptr(), dtype_code(w->scalar_type()), w->stride(0), &rq,
+                         scale.data_ptr<float>(), nullptr, static_cast<float>(eps), stream_of(*x)),
+          "fd_rms_fp8_out");
+  return py::make_tuple(q, scale);
+}
+
+py::object add_rms_norm_fp8(py::handle hx, py::handle hr, py::handle hw, py::handle heps, py::handle hout,
+                            py::handle hscale, py::handle hres_out) {
+  const at::Tensor* x = as_tensor(hx);
+  const at::Tensor* r = as_tensor(hr);
+  const at::Tensor* w = as_tensor(hw);
+  double eps;
+  fd_rows rx, rr, rq, rro;
+  if (!x || !r || !w || !activation(*x) || !same_meta(*r, *x) || !norm_weight_ok(*w, *x) || !eps_ok(heps, &eps) ||
+      !rows_of(*x, &rx) || !rows_of(*r, &rr))
+    return py::none();
+  const c10::cuda::CUDAGuard guard(x->device());
+  at::Tensor q, scale, res_out;
+  if (!rows8_for(hout, hscale, *x, &q, &scale, &rq) || !out_for(hres_out, *x, &res_out, &rro)) return py::none();
+  if (row_count(rx) > 0)
+    check(fd_rms_fp8_out(&rx, &rr, w->data_ptr(), dtype_code(w->scalar_type()), w->stride(0), &rq,
+                         scale.data_ptr<float>(), &rro, static_cast<float>(eps), stream_of(*x)),
+          "fd_rms_fp8_out");
+  return py::make_tuple(q, scale, res_out);
+}
+
+py::object swiglu_fp8(py::handle hg, py::handle hu, py::handle hout, py::handle hscale) {
+  const at::Tensor* g = as_tensor(hg);
+  const at::Tensor* u = as_tensor(hu);
+  fd_rows rg, ru, rq;
+  if (!g || !u || !activation(*g) || !same_meta(*u, *g) || !rows_of(*g, &rg) || !rows_of(*u, &ru)) return py::none();
+  const c10::cuda::CUDAGuard guard(g->device());
+  at::Tensor q, scale;
+  if (!rows8_for(hout, hscale, *g, &q, &scale, &rq)) return py::none();
+  if (row_count(rg) > 0)
+    check(fd_swiglu_fp8_out(&rg, &ru, &rq, scale.data_ptr<float>(), stream_of(*g)), "fd_swiglu_fp8_out");
+  return py::make_tuple(q, scale);
+}
+
+// ------------------------------------------------------------ products
+// The arguments linear_act and linear_fp8 share; false: not on the fast path.
+struct ProductCall {
+  int64_t m, n, k, sxm, sxk;
+  const void* bias = nullptr;
+  int bias_dt = 0;
+  int64_t sbias = 0;
+  const void* ra = nullptr;
+  int ra_dt = 0;
+  int64_t srm = 0, srn = 0;
+  int act = FD_ACT_NONE;
+  at::Tensor y;
+};
+
+bool act_of(py::handle h, int* act) {
+  if (h.is_none()) {
+    *act = FD_ACT_NONE;
+    return true;
+  }
+  if (!PyUnicode_Check(h.ptr())) return false;
+  const std::string s = py::cast<std::string>(h);
+  *act = s == "relu" ? FD_ACT_RELU : s == "silu" ? FD_ACT_SILU : s == "gelu" ? FD_ACT_GELU
+       : s == "gelu_tanh" ? FD_ACT_GELU_TANH : -1;
+  return *act >= 0;
+}
+
+bool product_call(const at::Tensor& x, const at::Tensor& w, py::handle hb, py::handle hact, py::handle hra,
+                  py::handle hout, at::ScalarType out_type, ProductCall* c) {
+  if (x.dim() < 1 || w.dim() != 2 || w.device() != x.device() || x.size(-1) != w.size(1) || !act_of(hact, &c->act))
+    return false;
+  c->n = w.size(0);
+  c->k = w.size(1);
+  if (!as_mk(x, &c->m, &c->sxm, &c->sxk) || c->m < 1 || c->n < 1 || c->k < 1) return false;
+  std::vector<int64_t> expected(x.sizes().begin(), x.sizes().end() - 1);
+  expected.push_back(c->n);
+  if (!hb.is_none()) {
+    const at::Tensor* b = as_tensor(hb);
+    if (!b || b->dim() != 1 || b->size(0) != c->n || b->device() != x.device() ||
+        (b->scalar_type() != out_type && b->scalar_type() != at::kFloat))
+      return false;
+    c->bias = b->data_ptr();
+    c->bias_dt = dtype_code(b->scalar_type());
+    c->sbias = b->stride(0);
+  }
+  if (!hra.is_none()) {
+    const at::Tensor* ra = as_tensor(hra);
+    if (!ra || ra->device() != x.device() || dtype_code(ra->scalar_type()) < 0) return false;
+    // the broadcasts of ops_fp8 that need no copy: a 1-D row, the contiguous
+    // full shape, and [1|M, 1|N] where the output has two dimensions
+    if (!(ra->dim() == 1 && ra->numel() == c->n) && ra->sizes() != c10::IntArrayRef(expected) && x.dim() != 2)
+      return false;
+    if (!row_add_strides(*ra, c->m, c->n, expected, &c->srm, &c->srn)) return false;
+    c->ra = ra->data_ptr();
+    c->ra_dt = dtype_code(ra->scalar_type());
+  }
+  if (hout.is_none()) {
+    c->y = at::empty(expected, x.options().dtype(out_type));
+    return true;
+  }
+  const at::Tensor* o = as_tensor(hout);
+  if (!o || o->sizes() != c10::IntArrayRef(expected) || o->scalar_type() != out_type || o->device() != x.device() ||
+      !o->is_contiguous())
+    return false;
+  c->y = *o;
+  return true;
+}
+
+py::object linear_act(py::handle hx, py::handle hw, py::handle hb, py::handle hact, py::handle hra, py::handle hout) {
+  const at::Tensor* x = as_tensor(hx);
+  const at::Tensor* w = as_tensor(hw);
+  if (!x || !w || !activation(*x) || w->scalar_type() != x->scalar_type()) return py::none();
+  const c10::cuda::CUDAGuard guard(x->device());
+  ProductCall c;
+  if (!product_call(*x, *w, hb, hact, hra, hout, x->scalar_type(), &c)) return py::none();
+  check(fd_linear_act_out(x->data_ptr(), c.sxm, c.sxk, w->data_ptr(), w->stride(0), w->stride(1), c.bias, c.bias_dt,
+                          c.sbias, c.ra, c.ra_dt, c.srm, c.srn, c.y.data_ptr(), c.n, 1, dtype_code(x->scalar_type()),
+                          c.act, c.m, c.n, c.k, stream_of(*x)),
+        "fd_linear_act_out");
+  return py::cast(c.y);
+}
+
+// An e4m3 operand and its scale: contiguous fp32 of shape `shape`.
+bool operand8(const at::Tensor* t, const at::Tensor* scale, c10::IntArrayRef shape) {
+  return t->is_cuda() && t->scalar_type() == at::kFloat8_e4m3fn && scale->scalar_type() == at::kFloat &&
+         scale->sizes() == shape && scale->is_contiguous() && scale->device() == t->device();
+}
+
+py::object linear_fp8(py::handle hx, py::handle hxs, py::handle hw, py::handle hws, py::handle hb, py::handle hact,
+                      py::handle hra, py::handle hout, bool bf16) {
+  const at::Tensor* x = as_tensor(hx);
+  const at::Tensor* xs = as_tensor(hxs);
+  const at::Tensor* w = as_tensor(hw);
+  const at::Tensor* ws = as_tensor(hws);
+  if (!x || !xs || !w || !ws || x->dim() < 1 || w->dim() != 2 ||
+      !operand8(x, xs, x->sizes().slice(0, x->dim() - 1)) || !operand8(w, ws, w->sizes().slice(0, 1)))
+    return py::none();
+  const c10::cuda::CUDAGuard guard(x->device());
+  const at::ScalarType out_type = bf16 ? at::kBFloat16 : at::kHalf;
+  ProductCall c;
+  if (!product_call(*x, *w, hb, hact, hra, hout, out_type, &c)) return py::none();
+  check(fd_linear_fp8_out(x->data_ptr(), c.sxm, c.sxk, xs->data_ptr<float>(), w->data_ptr(), w->stride(0),
+                          w->stride(1), ws->data_ptr<float>(), c.bias, c.bias_dt, c.sbias, c.ra, c.ra_dt, c.srm, c.srn,
+                          c.y.data_ptr(), c.n, 1, dtype_code(out_type), c.act, c.m, c.n, c.k, stream_of(*x)),
+        "fd_linear_fp8_out");
+  return py::cast(c.y);
+}
+
+py::object post_attn_mlp_fp8(py::handle hh, py::handle hnw, py::handle hgu, py::handle hgs, py::handle hd,
+                             py::handle hds, py::handle heps) {
+  const at::Tensor* hid = as_tensor(hh);
+  const at::Tensor* nw = as_tensor(hnw);
+  const at::Tensor* wgu = as_tensor(hgu);
+  const at::Tensor* gs = as_tensor(hgs);
+  const at::Tensor* wd = as_tensor(hd);
+  const at::Tensor* ds = as_tensor(hds);
+  double eps;
+  if (!hid || !nw || !wgu || !gs || !wd || !ds || !activation(*hid) || hid->dim() < 1 || wgu->dim() != 2 ||
+      wd->dim() != 2 || !eps_ok(heps, &eps) || !norm_weight_ok(*nw, *hid))
+    return py::none();
+  const int64_t h = wgu->size(1), i = wd->size(1);
+  if (wgu->size(0) != 2 * i || wd->size(0) != h || hid->size(-1) != h || h < 1 || i < 1) return py::none();
+  if (!operand8(wgu, gs, wgu->sizes().slice(0, 1)) || !operand8(wd, ds, wd->sizes().slice(0, 1)) ||
+      wgu->device() != hid->device() || wd->device() != hid->device() || wgu->stride(1) != 1 || wd->stride(1) != 1)
+    return py::none();
+  int64_t m, s_hidden, sxk;
+  if (!as_mk(*hid, &m, &s_hidden, &sxk) || m < 1 || sxk != 1) return py::none();
+  const c10::cuda::CUDAGuard guard(hid->device());
+  at::Tensor out = at::empty(hid->sizes(), hid->options());
+  const size_t bytes = fd_post_attn_mlp_fp8_workspace_bytes(m, h, i);
+  const at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, hid->options().dtype(at::kByte));
+  check(fd_post_attn_mlp_fp8_out(hid->data_ptr(), s_hidden, nw->data_ptr(), dtype_code(nw->scalar_type()),
+                                 nw->stride(0), wgu->data_ptr(), wgu->stride(0), gs->data_ptr<float>(), wd->data_ptr(),
+                                 wd->stride(0), ds->data_ptr<float>(), out.data_ptr(), dtype_code(hid->scalar_type()), m,
+                                 h, i, static_cast<float>(eps), ws.data_ptr(), bytes, stream_of(*hid)),
+        "fd_post_attn_mlp_fp8_out");
+  return py::cast(out);
+}
+
 // ------------------------------------------------------------ test hooks
 // The arguments the fast path derives from a tensor's layout, for any device,
 // so tests can compare them with the Python path's without a GPU.
@@ -479,6 +705,13 @@ PYBIND11_MODULE(_fastpath, mod) {
   mod.def("swiglu", &swiglu);
   mod.def("linear_decode", &linear_decode);
   mod.def("post_attn_mlp", &post_attn_mlp);
+  mod.def("quantize_fp8", &quantize_fp8);
+  mod.def("rms_norm_fp8", &rms_norm_fp8);
+  mod.def("add_rms_norm_fp8", &add_rms_norm_fp8);
+  mod.def("swiglu_fp8", &swiglu_fp8);
+  mod.def("linear_act", &linear_act);
+  mod.def("linear_fp8", &linear_fp8);
+  mod.def("post_attn_mlp_fp8", &post_attn_mlp_fp8);
   mod.def("layout_rows", &layout_rows);
   mod.def("layout_linear", &layout_linear);
   mod.def("workspace", &workspace);

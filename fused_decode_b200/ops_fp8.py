@@ -14,7 +14,8 @@ The 8-bit form of an fp32 row ``y``::
 to nearest even, saturating; a NaN in the row makes its scale NaN.  Inference
 only, any number of rows, no host synchronisation; like the rest of the
 package the operators launch on the current stream of their tensors' device
-and may be captured in a CUDA graph.
+and may be captured in a CUDA graph, and each first offers its arguments to
+the compiled dispatch (``_fastpath``), which takes the common case.
 """
 
 from __future__ import annotations
@@ -24,6 +25,7 @@ import math
 import torch
 
 from fused_decode_b200._capi import ACTIVATIONS
+from fused_decode_b200._capi import fast_or_none as _fast
 from fused_decode_b200.kernels import (
     linear_act_out,
     linear_fp8_out,
@@ -127,6 +129,10 @@ def quantize_fp8(
     Weights ``[N, K]`` are laid out with it once; activations that no operator
     here produces (the attention's output, say) on every step.
     """
+    fp = _fast()
+    done = fp.quantize_fp8(x, out, scale_out) if fp is not None else None
+    if done is not None:
+        return done
     _check_rows(x, "x")
     _check_rows8(out, scale_out, x)
     _check_device(x, "x", out=out, scale_out=scale_out)
@@ -148,6 +154,10 @@ def rms_norm_fp8(
     The fp32 rows are quantised directly, without the rounding to ``x``'s type
     that ``rms_norm`` makes.
     """
+    fp = _fast()
+    done = fp.rms_norm_fp8(x, weight, eps, out, scale_out) if fp is not None else None
+    if done is not None:
+        return done
     _check_rows(x, "x")
     eps = _check_norm(weight, x, eps)
     _check_rows8(out, scale_out, x)
@@ -172,6 +182,10 @@ def add_rms_norm_fp8(
     ``residual_out = x + residual`` in ``x``'s type; the norm sees the fp32
     sum.  Pass ``residual_out=residual`` to update the residual stream in place.
     """
+    fp = _fast()
+    done = fp.add_rms_norm_fp8(x, residual, weight, eps, out, scale_out, residual_out) if fp is not None else None
+    if done is not None:
+        return done
     _check_rows(x, "x")
     _check_like(residual, x, "residual")
     eps = _check_norm(weight, x, eps)
@@ -195,6 +209,10 @@ def swiglu_fp8(
 ) -> tuple[torch.Tensor, torch.Tensor]:
     """``silu(gate) * up`` in 8 bits: ``(values, scale)``.  ``gate`` and ``up``
     may be views, such as the halves of one gate/up product."""
+    fp = _fast()
+    done = fp.swiglu_fp8(gate, up, out, scale_out) if fp is not None else None
+    if done is not None:
+        return done
     _check_rows(gate, "gate")
     _check_like(up, gate, "up")
     _check_rows8(out, scale_out, gate)
@@ -275,6 +293,10 @@ def linear_act(
     both additions are fp32 and the result is rounded once.  ``out`` may be
     ``row_add`` itself.
     """
+    fp = _fast()
+    done = fp.linear_act(x, weight, bias, activation, row_add, out) if fp is not None else None
+    if done is not None:
+        return done
     _check_tensor(x, "x", _HALF, "float16 or bfloat16")
     _check_tensor(weight, "weight", (x.dtype,), str(x.dtype))
     expected = _check_product(x, weight, bias, activation, row_add, out, x.dtype)
@@ -307,6 +329,11 @@ def linear_fp8(
     ``quantize_fp8`` and its companions return them.  The output is of
     ``out_dtype`` (float16 or bfloat16), ``bias`` of that type or float32.
     """
+    fp = _fast() if out_dtype in _HALF else None
+    done = fp.linear_fp8(x, x_scale, weight, weight_scale, bias, activation, row_add, out,
+                         out_dtype == torch.bfloat16) if fp is not None else None
+    if done is not None:
+        return done
     _check_tensor(x, "x", (E4M3,), "float8_e4m3fn")
     _check_tensor(weight, "weight", (E4M3,), "float8_e4m3fn")
     if out_dtype not in _HALF:
@@ -345,6 +372,10 @@ def post_attn_mlp_fp8(
     -> ``linear_fp8`` -> ``swiglu_fp8`` -> ``linear_fp8`` with ``hidden`` as
     ``row_add``, enqueued by one call.
     """
+    fp = _fast()
+    done = fp.post_attn_mlp_fp8(hidden, norm_weight, w_gate_up, gate_up_scale, w_down, down_scale, eps) if fp is not None else None
+    if done is not None:
+        return done
     _check_rows(hidden, "hidden")
     for name, w in (("w_gate_up", w_gate_up), ("w_down", w_down)):
         _check_tensor(w, name, (E4M3,), "float8_e4m3fn")
