@@ -255,10 +255,43 @@ FD_DEV float ld_cluster_f32(uint32_t addr) {
   return v;
 }
 
+// Wait (bounded) for the phase of `bar` with this parity.  The bound is looked
+// at every 256 tries.  Acquiring at CTA scope is enough where the other CTA of
+// a pair signals, too: what these barriers pass on is shared-memory tiles
+// written by TMA and accumulators in tensor memory, never plain stores.
+constexpr int64_t kWaitClocks = 4000000000ll;  // 2 s at the highest clock
+FD_DEV bool wait_more(uint32_t addr, uint32_t parity) {
+  const int64_t t0 = clock64();
+  do {
+    for (int i = 0; i < 256; ++i)
+      if (fd_stream::mbar_try(addr, parity)) return true;
+  } while (clock64() - t0 < kWaitClocks);
+  return false;
+}
+FD_DEV bool wait_phase(uint64_t* bar, uint32_t parity) {
+  const uint32_t addr = fd_stream::smem_addr(bar);
+  return fd_stream::mbar_try(addr, parity) || wait_more(addr, parity);
+}
+
+// The ring stage of a role's next step, and how often the ring has come round:
+// counted up, since dividing the step number takes longer than a step.
+struct RingPos {
+  int stage = 0;
+  uint32_t phase = 0;
+  FD_DEV void next(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
+
 // A wait of one role: false once any role of this CTA has given up.
-FD_DEV bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort, bool cluster = false) {
+FD_DEV bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
+  const uint32_t addr = fd_stream::smem_addr(bar);
+  if (fd_stream::mbar_try(addr, parity)) return true;
   if (*abort) return false;
-  if (cluster ? fd_stream::mbar_wait_cluster(bar, parity) : fd_stream::mbar_wait(bar, parity)) return true;
+  if (wait_more(addr, parity)) return true;
   *abort = 1;
   atomicOr(&g_product_status, kStatusWait);
   return false;
@@ -348,10 +381,11 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       const int32_t row = static_cast<int32_t>(warp == 0 ? n0 : m0);
       const uint64_t policy = evict_first_policy();
       if (warp == 1 || !a.w_early) grid_dep_wait();
+      RingPos p;
       int i = 0;
-      for (; i < count; ++i) {
-        const int s = i % a.stages;
-        if (i >= a.stages && !wait_or_abort(&empty[s], (i / a.stages - 1) & 1, &abort)) break;
+      for (; i < count; ++i, p.next(a.stages)) {
+        const int s = p.stage;
+        if (i >= a.stages && !wait_or_abort(&empty[s], p.phase ^ 1, &abort)) break;
         uint8_t* dst = ring + static_cast<size_t>(s) * stage_bytes + (warp == 0 ? 0 : wbytes);
         mbar_expect_tx(&full[s], bytes);
         for (int b = 0; b < a.boxes; ++b) {
@@ -363,16 +397,17 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       // every copy of this CTA has landed and been read before it may exit
       bool read = true;
       for (int j = i > a.stages ? i - a.stages : 0; j < i; ++j) {
-        read = read && mbar_wait(&empty[j % a.stages], (j / a.stages) & 1);
-        if (!read) mbar_wait(&full[j % a.stages], (j / a.stages) & 1);
+        read = read && wait_phase(&empty[j % a.stages], (j / a.stages) & 1);
+        if (!read) wait_phase(&full[j % a.stages], (j / a.stages) & 1);
       }
     }
     __syncwarp();
   } else if (warp == 2) {
     if (lane == 0) {
-      for (int i = 0; i < count; ++i) {
-        const int s = i % a.stages;
-        if (!wait_or_abort(&full[s], (i / a.stages) & 1, &abort)) break;
+      RingPos p;
+      for (int i = 0; i < count; ++i, p.next(a.stages)) {
+        const int s = p.stage;
+        if (!wait_or_abort(&full[s], p.phase, &abort)) break;
         tc_fence_after();
         const uint32_t w = smem_addr(ring + static_cast<size_t>(s) * stage_bytes), x = w + wbytes;
         for (int b = 0; b < a.boxes; ++b)
@@ -540,6 +575,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     if (lane == 0) {
       prefetch_map(&xmap);
       prefetch_map(&wmap);
+      const uint32_t bars = cluster_map(full, 0);
+      RingPos p;
       int64_t i = 0;
       bool ok = true;
       for (int64_t t = first; t < tiles && ok; t += pairs) {
@@ -547,15 +584,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         pair_tile(a, t, &mi, &ni);
         const int32_t xr = static_cast<int32_t>(mi * kPairRows + rank * 128);
         const int32_t wr = static_cast<int32_t>(ni * a.cols + rank * half_cols);
-        for (int k = 0; k < a.steps; ++k, ++i) {
-          const int s = static_cast<int>(i % a.stages);
-          if (i >= a.stages && !wait_or_abort(&empty[s], (i / a.stages - 1) & 1, &abort, true)) {
+        for (int k = 0; k < a.steps; ++k, ++i, p.next(a.stages)) {
+          const int s = p.stage;
+          if (i >= a.stages && !wait_or_abort(&empty[s], p.phase ^ 1, &abort)) {
             ok = false;
             break;
           }
           // the first CTA's barrier counts the bytes of both
           if (rank == 0) mbar_expect_tx(&full[s], 2 * stage_bytes);
-          const uint32_t bar = cluster_map(&full[s], 0);
+          const uint32_t bar = bars + s * 8;
           uint8_t* dst = ring + static_cast<size_t>(s) * stage_bytes;
           tma_load_pair(dst, &xmap, k * a.box_elems, xr, bar);
           tma_load_pair(dst + xbytes, &wmap, k * a.box_elems, wr, bar);
@@ -564,24 +601,24 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       // every stage has landed and been read, and its barrier signalled, before the pair may exit
       bool read = true;
       for (int64_t j = i > a.stages ? i - a.stages : 0; j < i; ++j) {
-        read = read && mbar_wait_cluster(&empty[j % a.stages], (j / a.stages) & 1);
-        if (!read && rank == 0) mbar_wait_cluster(&full[j % a.stages], (j / a.stages) & 1);
+        read = read && wait_phase(&empty[j % a.stages], (j / a.stages) & 1);
+        if (!read && rank == 0) wait_phase(&full[j % a.stages], (j / a.stages) & 1);
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
-      int64_t i = 0;
+      RingPos p;
       int it = 0;
       bool ok = true;
       for (int64_t t = first; t < tiles && ok; t += pairs, ++it) {
         const int b = it & 1;
-        if (!wait_or_abort(&acc_empty[b], ((it >> 1) & 1) ^ 1, &abort, true)) break;
+        if (!wait_or_abort(&acc_empty[b], ((it >> 1) & 1) ^ 1, &abort)) break;
         tc_fence_after();
         const uint32_t d = tmem + b * kPairCols;
-        for (int k = 0; k < a.steps; ++k, ++i) {
-          const int s = static_cast<int>(i % a.stages);
-          if (!wait_or_abort(&full[s], (i / a.stages) & 1, &abort, true)) {
+        for (int k = 0; k < a.steps; ++k, p.next(a.stages)) {
+          const int s = p.stage;
+          if (!wait_or_abort(&full[s], p.phase, &abort)) {
             ok = false;
             break;
           }
@@ -616,7 +653,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const float xs = FP8 && m < a.e.m ? a.e.xs[m] : 1.f;
       named_sync(1, 128);
       // after an expired wait the four warps still meet at every tile's barrier
-      ok = __all_sync(0xffffffffu, ok && wait_or_abort(&acc_full[b], (it >> 1) & 1, &abort, true));
+      ok = __all_sync(0xffffffffu, ok && wait_or_abort(&acc_full[b], (it >> 1) & 1, &abort));
       if (!ok) continue;
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kPairCols;
@@ -818,14 +855,23 @@ int launch_pair(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t 
       a.cols = c;
     }
   }
+  a.group = 8;
+  int max_stages = kMaxRing;
+  if (const char* env = std::getenv("FD_PAIR_TUNE")) {
+    int b = 0, c = 0, d = 0;
+    if (std::sscanf(env, "%d,%d,%d", &b, &c, &d) == 3) {
+      if (b > 0) a.cols = b;
+      if (c > 0) a.group = c;
+      if (d > 0) max_stages = d;
+    }
+  }
   a.nt = (e.n + a.cols - 1) / a.cols;
   if (steps > 0x7fffffffLL || e.m > 0x7fffff00LL || e.n > 0x7fffff00LL) return FD_ERR_UNSUPPORTED;
   a.steps = static_cast<int32_t>(steps);
-  a.group = 8;
   a.desc = mma_desc(FP8 ? 0 : mma_format(in_dtype), kPairRows, a.cols);
   a.vec = epilogue_vec(e, out_dtype);
   const size_t stage = static_cast<size_t>(kBoxBytes) * (128 + a.cols / 2);
-  a.stages = static_cast<int32_t>(std::min<size_t>(kMaxRing, 192 * 1024 / stage));
+  a.stages = static_cast<int32_t>(std::min<size_t>(max_stages, 192 * 1024 / stage));
   const size_t smem = a.stages * stage + 1024;
   CUtensorMap xm, wm;
   if (!operand_map(&xm, g.x, e.m, g.k, g.sxm, g.sxk, es, 128) ||
