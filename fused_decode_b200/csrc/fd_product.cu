@@ -7,6 +7,9 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
+#include <map>
+#include <mutex>
+#include <tuple>
 
 using namespace fd;
 
@@ -153,7 +156,7 @@ __global__ void __launch_bounds__(128) product_generic_kernel(GenericArgs a) {
 // K, in shared-memory tiles of 128-byte rows (64 16-bit or 128 8-bit elements)
 // with the 128-byte swizzle TMA writes; one instruction takes 32 bytes of K.
 constexpr int kBoxBytes = 128;  // K bytes of a tile row
-constexpr int kMaxRing = 10;
+constexpr int kMaxRing = 12;
 constexpr int kSliceBytes = 32;  // K bytes of one tcgen05.mma
 
 constexpr int kStatusWait = 1;  // a bounded wait expired: the call's output is invalid
@@ -212,9 +215,9 @@ FD_DEV void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) 
 #undef FD_TC_MMA
 }
 // Arrive on `bar` once every earlier MMA of this thread has completed; with
-// two CTAs, on the same barrier of both.
+// two CTAs, on the same barrier of the cluster's CTAs in `mask`.
 template <int CTAS>
-FD_DEV void tc_commit(uint64_t* bar) {
+FD_DEV void tc_commit(uint64_t* bar, uint16_t mask = 0) {
   if constexpr (CTAS == 1)
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
                      fd_stream::smem_addr(bar))
@@ -223,7 +226,7 @@ FD_DEV void tc_commit(uint64_t* bar) {
     asm volatile(
         "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
             fd_stream::smem_addr(bar)),
-        "h"(static_cast<uint16_t>(3))
+        "h"(mask)
         : "memory");
 }
 
@@ -247,11 +250,39 @@ FD_DEV void tc_load32(uint32_t addr, uint32_t* v) {
       : "memory");
 }
 
+// One lane of a converged warp, chosen by elect.sync.  TMA and tcgen05
+// instructions take warp-uniform operands; issued under `if (lane == 0)`
+// instead, a step of four MMAs and its commit measured about 700 cycles whatever
+// the tile, under elect.sync as little as its MMAs take (4096 x 14336 x 4096 in
+// 16 bits: 340 -> 312 us, 1 x 28672 x 4096: 59 -> 49 us).
+FD_DEV bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.b32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one != 0;
+}
+FD_DEV int warp_index() { return __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0); }
+
+// Bring a tile into L2 only.  L2 is where all SMs' accesses meet, so this may run
+// before the kernel that writes the tile has finished.
+FD_DEV void tma_prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
+  asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y)
+               : "memory");
+}
+
 FD_DEV void bar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 FD_DEV void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 FD_DEV float ld_cluster_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+FD_DEV float4 ld_cluster_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr)
+               : "memory");
   return v;
 }
 
@@ -276,8 +307,8 @@ FD_DEV bool wait_phase(uint64_t* bar, uint32_t parity) {
 // The ring stage of a role's next step, and how often the ring has come round:
 // counted up, since dividing the step number takes longer than a step.
 struct RingPos {
-  int stage = 0;
-  uint32_t phase = 0;
+  int stage;
+  uint32_t phase;
   FD_DEV void next(int stages) {
     if (++stage == stages) {
       stage = 0;
@@ -286,14 +317,38 @@ struct RingPos {
   }
 };
 
-// A wait of one role: false once any role of this CTA has given up.
+FD_DEV bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort);
+
+// Wait for the step at `p`, and look at the ring's later stages with the other
+// lanes: how many steps in a row (at most `most`) have arrived, 0 once any role
+// has given up.  One look costs about 150 ns, as much as issuing a step's MMAs.
+FD_DEV int wait_steps(uint64_t* bars, RingPos p, int stages, int most, volatile int* abort) {
+  const int lane = threadIdx.x & 31;
+  most = min(most, stages);
+  int s = p.stage + lane;
+  uint32_t phase = p.phase;
+  if (s >= stages) {
+    s -= stages;
+    phase ^= 1;
+  }
+  const uint32_t addr = fd_stream::smem_addr(bars + (lane < most ? s : p.stage));
+  if (lane >= most) phase = p.phase;
+  uint32_t here = __ballot_sync(0xffffffffu, fd_stream::mbar_try(addr, phase));
+  if (!(here & 1)) {
+    if (!wait_or_abort(bars + p.stage, p.phase, abort)) return 0;
+    here = 1;
+  }
+  return min(here == 0xffffffffu ? 32 : __ffs(~here) - 1, most);
+}
+
+// A warp's wait: false, for all of its lanes, once any role of this CTA has given up.
 FD_DEV bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort) {
   const uint32_t addr = fd_stream::smem_addr(bar);
-  if (fd_stream::mbar_try(addr, parity)) return true;
-  if (*abort) return false;
-  if (wait_more(addr, parity)) return true;
+  bool done = fd_stream::mbar_try(addr, parity);
+  if (!done && !*abort) done = wait_more(addr, parity);
+  if (__all_sync(0xffffffffu, done)) return true;
   *abort = 1;
-  atomicOr(&g_product_status, kStatusWait);
+  if ((threadIdx.x & 31) == 0) atomicOr(&g_product_status, kStatusWait);
   return false;
 }
 
@@ -314,30 +369,62 @@ FD_DEV void activate_all(float* v, int act) {
 }
 
 // ============================================================== few rows
-// Weight-stationary tiles for products bound by the weight's bytes: 128 rows
-// of w are the MMA's rows, up to 256 rows of x (a multiple of 16) its columns,
-// and the K steps of a tile are divided among the CTAs of a thread-block
-// cluster.  Each CTA streams its part of the tile through a TMA ring (one warp
-// for w, one for x, one issuing MMAs), the partial tiles meet through
-// distributed shared memory, where every CTA sums some columns of all partials
-// in rank order: the same bits every time, and no workspace that two streams
-// or graphs could share.
-constexpr int kTileRows = 128;
+// Products bound by the weight's bytes.  The weight's rows are cut into tiles
+// of R rows (any multiple of 8 up to 256) so that the tiles, or the tiles times
+// the CTAs that share the K steps of each, number the SMs: every SM streams
+// the same share of the weight.  A tile's rows are the MMA's rows (one or two
+// blocks of 128; rows beyond R are whatever shared memory holds, and nothing
+// reads their sums), up to 80 rows of x its columns.  Each CTA streams its part
+// through a TMA ring (one warp for w, one for x, one issuing MMAs).  Where a
+// thread-block cluster shares a tile's K steps, the partial tiles meet through
+// distributed shared memory and every CTA sums some columns of all partials in
+// rank order: the same bits every time, and no workspace that two streams or
+// graphs could share.  Otherwise a CTA goes over several tiles where there are
+// more than SMs, the epilogue of one under the stream of the next.
+constexpr int kBlockRows = 128;  // rows of one MMA
 constexpr int kSplitThreads = 256;
 constexpr int kMaxSplit = 8;
 
 struct SplitArgs {
   Epilogue e;
-  int32_t steps;   // K steps of a tile (boxes * 128 bytes each)
-  int32_t cols;    // rows of x per tile (MMA columns)
-  int32_t boxes;   // 128-byte boxes per step
+  int64_t tiles;
+  int32_t rows;    // R
+  int32_t blocks;  // MMA row blocks per tile
+  int32_t cols;    // rows of x, rounded up to 16 (MMA columns)
+  int32_t steps;   // K steps of a tile, 128 bytes each
   int32_t stages;
   int32_t split;   // CTAs per tile
+  int32_t accs;    // accumulators (2: the epilogue overlaps the next tile)
   int32_t box_elems;
   uint32_t desc;
   uint32_t tmem_cols;
-  int32_t w_early;  // the kernel before this one does not write w
+  int32_t ahead;   // steps of w brought into L2 before the kernel before this one has finished
+  int32_t vec;     // y and row_add take 4 columns at a time
 };
+
+// Four consecutive columns of y from their sums.
+template <typename T, bool FP8>
+FD_DEV void finish4(const SplitArgs& a, int64_t m, int64_t n, const float* sum) {
+  if (!a.vec || n + 4 > a.e.n) {
+    for (int j = 0; j < 4 && n + j < a.e.n; ++j) finish<T, FP8>(a.e, m, n + j, sum[j]);
+    return;
+  }
+  float v[4];
+  const float xs = FP8 ? a.e.xs[m] : 1.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j] = FP8 ? sum[j] * xs * a.e.ws[n + j] : sum[j];
+    if (a.e.bias) v[j] += load_as_f32(a.e.bias, a.e.bias_dtype, (n + j) * a.e.sbias);
+  }
+  activate_all<4>(v, a.e.act);
+  if (a.e.ra) {
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.e.ra) + m * a.e.srm + n);
+    const float2 lo = unpack2<T>(w.x), hi = unpack2<T>(w.y);
+    v[0] += lo.x; v[1] += lo.y; v[2] += hi.x; v[3] += hi.y;
+  }
+  *reinterpret_cast<uint2*>(static_cast<T*>(a.e.y) + m * a.e.sym + n) =
+      make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+}
 
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(kSplitThreads, 1)
@@ -345,25 +432,27 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
                          const __grid_constant__ SplitArgs a) {
   using namespace fd_stream;
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t full[kMaxRing], empty[kMaxRing], done;
+  __shared__ uint64_t full[kMaxRing], empty[kMaxRing], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort;
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const uint32_t rank = a.split > 1 ? cluster_ctarank() : 0;
-  const int64_t n0 = static_cast<int64_t>(blockIdx.x / a.split) * kTileRows;
-  const int64_t m0 = static_cast<int64_t>(blockIdx.y) * a.cols;
+  const int64_t first = blockIdx.x / a.split, stride = gridDim.x / a.split;
   const int s0 = static_cast<int>(static_cast<int64_t>(rank) * a.steps / a.split);
   const int count = static_cast<int>(static_cast<int64_t>(rank + 1) * a.steps / a.split) - s0;
-  const uint32_t wbytes = a.boxes * kTileRows * kBoxBytes, xbytes = a.boxes * a.cols * kBoxBytes;
-  const uint32_t stage_bytes = wbytes + xbytes;
+  const uint32_t wbytes = a.rows * kBoxBytes, xbytes = a.cols * kBoxBytes, stage_bytes = wbytes + xbytes;
+  const uint32_t acc_cols = a.blocks * a.cols;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
       mbar_init(&full[s], 2);
       mbar_init(&empty[s], 1);
     }
-    mbar_init(&done, 1);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 4);
+    }
     abort = 0;
     bar_init_fence();
   }
@@ -374,110 +463,162 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   const uint32_t tmem = tmem_slot;
 
   if (warp <= 1) {
-    if (lane == 0) {
-      const CUtensorMap* map = warp == 0 ? &wmap : &xmap;
-      prefetch_map(map);
-      const uint32_t bytes = warp == 0 ? wbytes : xbytes, box = bytes / a.boxes;
-      const int32_t row = static_cast<int32_t>(warp == 0 ? n0 : m0);
-      const uint64_t policy = evict_first_policy();
-      if (warp == 1 || !a.w_early) grid_dep_wait();
-      RingPos p;
-      int i = 0;
-      for (; i < count; ++i, p.next(a.stages)) {
-        const int s = p.stage;
-        if (i >= a.stages && !wait_or_abort(&empty[s], p.phase ^ 1, &abort)) break;
-        uint8_t* dst = ring + static_cast<size_t>(s) * stage_bytes + (warp == 0 ? 0 : wbytes);
-        mbar_expect_tx(&full[s], bytes);
-        for (int b = 0; b < a.boxes; ++b) {
-          const int32_t col = ((s0 + i) * a.boxes + b) * a.box_elems;
-          if (warp == 0) tma_load_2d(dst + b * box, map, col, row, &full[s], policy);
-          else tma_load_2d_plain(dst + b * box, map, col, row, &full[s]);
+    const CUtensorMap* map = warp == 0 ? &wmap : &xmap;
+    const uint32_t bytes = warp == 0 ? wbytes : xbytes;
+    const uint64_t policy = evict_first_policy();
+    if (elect_one()) prefetch_map(map);
+    grid_dep_wait();
+    RingPos p{0, 0};
+    int64_t i = 0;
+    bool ok = true;
+    for (int64_t t = first; t < a.tiles && ok; t += stride) {
+      const int32_t row = warp == 0 ? static_cast<int32_t>(t * a.rows) : 0;
+      for (int k = 0; k < count; ++k, ++i, p.next(a.stages)) {
+        if (i >= a.stages && !wait_or_abort(&empty[p.stage], p.phase ^ 1, &abort)) {
+          ok = false;
+          break;
         }
+        uint8_t* dst = ring + p.stage * stage_bytes + (warp == 0 ? 0 : wbytes);
+        if (elect_one()) {
+          mbar_expect_tx(&full[p.stage], bytes);
+          if (warp == 0) tma_load_2d(dst, map, (s0 + k) * a.box_elems, row, &full[p.stage], policy);
+          else tma_load_2d_plain(dst, map, (s0 + k) * a.box_elems, row, &full[p.stage]);
+        }
+        __syncwarp();
       }
-      // every copy of this CTA has landed and been read before it may exit
-      bool read = true;
-      for (int j = i > a.stages ? i - a.stages : 0; j < i; ++j) {
-        read = read && wait_phase(&empty[j % a.stages], (j / a.stages) & 1);
-        if (!read) wait_phase(&full[j % a.stages], (j / a.stages) & 1);
-      }
+    }
+    // every copy of this CTA has landed and been read before it may exit
+    bool read = true;
+    for (int64_t j = i > a.stages ? i - a.stages : 0; j < i; ++j) {
+      read = read && wait_phase(&empty[j % a.stages], (j / a.stages) & 1);
+      if (!read) wait_phase(&full[j % a.stages], (j / a.stages) & 1);
     }
     __syncwarp();
   } else if (warp == 2) {
-    if (lane == 0) {
-      RingPos p;
-      for (int i = 0; i < count; ++i, p.next(a.stages)) {
-        const int s = p.stage;
-        if (!wait_or_abort(&full[s], p.phase, &abort)) break;
+    const uint64_t ring_desc = tile_desc(smem_addr(ring));  // addresses in 16-byte units: below 2^14
+    RingPos p{0, 0};
+    bool ok = true;
+    int it = 0;
+    for (int64_t t = first; t < a.tiles && ok; t += stride, ++it) {
+      const int b = a.accs == 2 ? it & 1 : 0, turn = a.accs == 2 ? it >> 1 : it;
+      if (!wait_or_abort(&acc_empty[b], (turn & 1) ^ 1, &abort)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + b * acc_cols;
+      for (int k = 0; k < count;) {
+        const int here = wait_steps(full, p, a.stages, count - k, &abort);
+        if (here == 0) {
+          ok = false;
+          break;
+        }
         tc_fence_after();
-        const uint32_t w = smem_addr(ring + static_cast<size_t>(s) * stage_bytes), x = w + wbytes;
-        for (int b = 0; b < a.boxes; ++b)
+        for (int j = 0; j < here; ++j, ++k, p.next(a.stages)) {
+          const uint64_t w = ring_desc + p.stage * (stage_bytes / 16), x = w + wbytes / 16;
+          if (elect_one()) {
+            for (int r = 0; r < a.blocks; ++r)
 #pragma unroll
-          for (int k = 0; k < kBoxBytes; k += kSliceBytes)
-            tc_mma<FP8, 1>(tmem, tile_desc(w + b * kTileRows * kBoxBytes + k), tile_desc(x + b * a.cols * kBoxBytes + k),
-                           a.desc, i + b + k > 0);
-        tc_commit<1>(&empty[s]);
+              for (int kk = 0; kk < kBoxBytes; kk += kSliceBytes)
+                tc_mma<FP8, 1>(d + r * a.cols, w + (r * kBlockRows * kBoxBytes + kk) / 16, x + kk / 16, a.desc,
+                               k + kk > 0);
+            tc_commit<1>(&empty[p.stage]);
+            if (k + 1 == count) tc_commit<1>(&acc_full[b]);
+          }
+          __syncwarp();
+        }
       }
-      tc_commit<1>(&done);
     }
+  } else if (warp == 3) {
+    for (int i = 0; i < min(count, a.ahead); ++i)
+      if (elect_one()) tma_prefetch_2d(&wmap, (s0 + i) * a.box_elems, static_cast<int32_t>(first * a.rows));
     __syncwarp();
   }
   grid_dep_wait();
   grid_dep_launch();
-  const bool ok = __all_sync(0xffffffffu, wait_or_abort(&done, 0, &abort));
-  tc_fence_after();
-  const int live = static_cast<int>(min(static_cast<int64_t>(a.cols), a.e.m - m0));  // columns in use
-  const int r = threadIdx.x & (kTileRows - 1);
-  const int64_t n = n0 + r;
-  const bool row_ok = n < a.e.n;
-  const float ws = FP8 && row_ok ? a.e.ws[n] : 1.f;
-  const float bias = a.e.bias && row_ok ? load_as_f32(a.e.bias, a.e.bias_dtype, n * a.e.sbias) : 0.f;
-  auto store = [&](int64_t m, float v) {
-    if (FP8) v = v * a.e.xs[m] * ws;
-    v = activate(v + bias, a.e.act);
-    if (a.e.ra) v += load_as_f32(a.e.ra, a.e.ra_dtype, m * a.e.srm + n * a.e.srn);
-    static_cast<T*>(a.e.y)[m * a.e.sym + n * a.e.syn] = from_f32<T>(v);
-  };
+  const int live = static_cast<int>(a.e.m);  // columns in use
   if (a.split == 1) {
-    if (warp >= 4 && ok) {
-      const uint32_t mine = tmem + (static_cast<uint32_t>(r & ~31) << 16);
-      for (int c = 0; c < live; c += 16) {
-        uint32_t v[16];
-        tc_load16(mine + c, v);
-        if (row_ok) {
+    // straight from tensor memory: a thread per row of the tile
+    if (warp >= 4) {
+      bool ok = true;
+      int it = 0;
+      for (int64_t t = first; t < a.tiles; t += stride, ++it) {
+        const int b = a.accs == 2 ? it & 1 : 0, turn = a.accs == 2 ? it >> 1 : it;
+        ok = ok && wait_or_abort(&acc_full[b], turn & 1, &abort);
+        if (!ok) break;
+        tc_fence_after();
+        for (int blk = 0; blk < a.blocks; ++blk) {
+          const int r = blk * kBlockRows + (warp - 4) * 32 + lane;
+          const int64_t n = t * a.rows + r;
+          const bool row_ok = r < a.rows && n < a.e.n;
+          const float ws = FP8 && row_ok ? a.e.ws[n] : 1.f;
+          const float bias = a.e.bias && row_ok ? load_as_f32(a.e.bias, a.e.bias_dtype, n * a.e.sbias) : 0.f;
+          const uint32_t acc = tmem + (static_cast<uint32_t>((warp - 4) * 32) << 16) + b * acc_cols + blk * a.cols;
+          for (int c = 0; c < live; c += 16) {
+            float v[16];
+            tc_load16(acc + c, reinterpret_cast<uint32_t*>(v));
+            if (!row_ok) continue;
 #pragma unroll
-          for (int j = 0; j < 16; ++j)
-            if (c + j < live) store(m0 + c + j, __uint_as_float(v[j]));
+            for (int j = 0; j < 16; ++j)
+              v[j] = (FP8 ? v[j] * (c + j < live ? a.e.xs[c + j] : 0.f) * ws : v[j]) + bias;
+            activate_all<16>(v, a.e.act);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int64_t m = c + j;
+              if (m >= live) break;
+              if (a.e.ra) v[j] += load_as_f32(a.e.ra, a.e.ra_dtype, m * a.e.srm + n * a.e.srn);
+              static_cast<T*>(a.e.y)[m * a.e.sym + n * a.e.syn] = from_f32<T>(v[j]);
+            }
+          }
+          __syncwarp();
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&acc_empty[b]);
       }
     }
   } else {
-    // partial tiles in the ring's memory, a column of 128 floats after another
+    // partial tiles in the ring's memory, a column of R floats after another
     float* part = reinterpret_cast<float*>(ring);
+    const bool ok = wait_or_abort(&acc_full[0], 0, &abort);
+    tc_fence_after();
     if (warp >= 4 && ok) {
-      const uint32_t mine = tmem + (static_cast<uint32_t>(r & ~31) << 16);
-      for (int c = 0; c < live; c += 16) {
-        uint32_t v[16];
-        tc_load16(mine + c, v);
+      for (int blk = 0; blk < a.blocks; ++blk) {
+        const int r = blk * kBlockRows + (warp - 4) * 32 + lane;
+        const uint32_t acc = tmem + (static_cast<uint32_t>((warp - 4) * 32) << 16) + blk * a.cols;
+        for (int c = 0; c < live; c += 16) {
+          uint32_t v[16];
+          tc_load16(acc + c, v);
+          if (r < a.rows) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          if (c + j < live) part[(c + j) * kTileRows + r] = __uint_as_float(v[j]);
+            for (int j = 0; j < 16; ++j)
+              if (c + j < live) part[(c + j) * a.rows + r] = __uint_as_float(v[j]);
+          }
+        }
+        __syncwarp();
       }
     }
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    if (row_ok) {
-      for (int c = static_cast<int>(rank) + a.split * (threadIdx.x / kTileRows); c < live;
-           c += a.split * (kSplitThreads / kTileRows)) {
-        float v = 0.f;
-        for (int p = 0; p < a.split; ++p) v += ld_cluster_f32(cluster_map(part + c * kTileRows + r, p));
-        store(m0 + c, v);
+    const int quads = a.rows / 4;
+    const int mine = live > static_cast<int>(rank) ? (live - static_cast<int>(rank) - 1) / a.split + 1 : 0;  // columns
+    for (int i = threadIdx.x; i < mine * quads; i += kSplitThreads) {
+      const int c = static_cast<int>(rank) + i / quads * a.split, r = i % quads * 4;
+      float4 from[kMaxSplit];  // all on their way before the first is added
+#pragma unroll
+      for (int p = 0; p < kMaxSplit; ++p)
+        from[p] = p < a.split ? ld_cluster_f4(cluster_map(part + c * a.rows + r, p)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int p = 0; p < kMaxSplit; ++p) {
+        v[0] += from[p].x; v[1] += from[p].y; v[2] += from[p].z; v[3] += from[p].w;
       }
+      const int64_t n = first * a.rows + r;
+      if (n < a.e.n) finish4<T, FP8>(a, c, n, v);
     }
     __syncwarp();
     cluster_arrive();  // the other CTAs may still be reading this one's partial
     cluster_wait();
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 3) {
@@ -503,6 +644,7 @@ struct PairArgs {
   int32_t steps;  // 128-byte boxes along K
   int32_t cols;   // rows of w per tile
   int32_t stages;
+  int32_t split;  // pairs that share a tile
   int32_t box_elems;
   uint32_t desc;
   int64_t mt, nt;  // tiles along m and n
@@ -531,6 +673,51 @@ FD_DEV void arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
+// Columns c .. c + 31 of 32 rows of a tile, from their sums: lane l holds row m0 + l.
+template <typename T, bool FP8>
+FD_DEV void emit_chunk(const PairArgs& a, float* v, int64_t m0, int64_t n0, float xs, const float* ws, const float* bias,
+                       float* stage) {
+  const int lane = threadIdx.x & 31;
+  const int64_t m = m0 + lane;
+#pragma unroll
+  for (int j = 0; j < kChunk; ++j) {
+    if (FP8) v[j] = v[j] * xs * ws[j];
+    v[j] += bias[j];
+  }
+  activate_all<kChunk>(v, a.e.act);
+  if (a.vec) {
+    if (m >= a.e.m) return;
+    T* y = static_cast<T*>(a.e.y) + m * a.e.sym + n0;
+    const T* ra = static_cast<const T*>(a.e.ra) + (a.e.ra ? m * a.e.srm + n0 : 0);
+#pragma unroll
+    for (int j = 0; j < kChunk; j += 8) {
+      if (n0 + j >= a.e.n) break;
+      if (a.e.ra) {
+        float f[8];
+        unpack8<T>(*reinterpret_cast<const uint4*>(ra + j), f);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[j + u] += f[u];
+      }
+      *reinterpret_cast<uint4*>(y + j) = pack8<T>(v + j);
+    }
+    return;
+  }
+  // any layout of y and row_add: through shared memory, a row of 32
+  // consecutive columns at a time
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < kChunk; ++j) stage[lane * kStagePitch + j] = v[j];
+  __syncwarp();
+  const int64_t n = n0 + lane;
+  if (n < a.e.n) {
+    for (int r = 0; r < 32 && m0 + r < a.e.m; ++r) {
+      float o = stage[r * kStagePitch + lane];
+      if (a.e.ra) o += load_as_f32(a.e.ra, a.e.ra_dtype, (m0 + r) * a.e.srm + n * a.e.srn);
+      static_cast<T*>(a.e.y)[(m0 + r) * a.e.sym + n * a.e.syn] = from_f32<T>(o);
+    }
+  }
+}
+
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(kPairThreads, 1)
     product_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
@@ -543,11 +730,15 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   __shared__ __align__(16) float s_bias[2][kPairCols], s_ws[2][kPairCols];
   __shared__ float s_stage[4][32 * kStagePitch];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_ctarank();
+  const int warp = warp_index(), lane = threadIdx.x & 31;
+  // a cluster's CTAs: pairs of neighbours, the first of a pair issues its MMAs
+  const uint32_t crank = cluster_ctarank(), side = crank & 1, pair = crank >> 1;
+  const uint16_t both = static_cast<uint16_t>(3u << (pair * 2));
   const int half_cols = a.cols / 2;
   const uint32_t xbytes = 128 * kBoxBytes, wbytes = half_cols * kBoxBytes, stage_bytes = xbytes + wbytes;
-  const int64_t tiles = a.mt * a.nt, pairs = gridDim.x / 2, first = blockIdx.x / 2;
+  const int64_t tiles = a.mt * a.nt, stride = gridDim.x / (2 * a.split), first = blockIdx.x / (2 * a.split);
+  const int s0 = static_cast<int>(static_cast<int64_t>(pair) * a.steps / a.split);
+  const int count = static_cast<int>(static_cast<int64_t>(pair + 1) * a.steps / a.split) - s0;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
@@ -572,77 +763,84 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   grid_dep_launch();
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       prefetch_map(&xmap);
       prefetch_map(&wmap);
-      const uint32_t bars = cluster_map(full, 0);
-      RingPos p;
-      int64_t i = 0;
-      bool ok = true;
-      for (int64_t t = first; t < tiles && ok; t += pairs) {
-        int64_t mi, ni;
-        pair_tile(a, t, &mi, &ni);
-        const int32_t xr = static_cast<int32_t>(mi * kPairRows + rank * 128);
-        const int32_t wr = static_cast<int32_t>(ni * a.cols + rank * half_cols);
-        for (int k = 0; k < a.steps; ++k, ++i, p.next(a.stages)) {
-          const int s = p.stage;
-          if (i >= a.stages && !wait_or_abort(&empty[s], p.phase ^ 1, &abort)) {
-            ok = false;
-            break;
-          }
-          // the first CTA's barrier counts the bytes of both
-          if (rank == 0) mbar_expect_tx(&full[s], 2 * stage_bytes);
-          const uint32_t bar = bars + s * 8;
-          uint8_t* dst = ring + static_cast<size_t>(s) * stage_bytes;
-          tma_load_pair(dst, &xmap, k * a.box_elems, xr, bar);
-          tma_load_pair(dst + xbytes, &wmap, k * a.box_elems, wr, bar);
+    }
+    const uint32_t bars = cluster_map(full, crank - side);
+    RingPos p{0, 0};
+    int64_t i = 0;
+    bool ok = true;
+    for (int64_t t = first; t < tiles && ok; t += stride) {
+      int64_t mi, ni;
+      pair_tile(a, t, &mi, &ni);
+      const int32_t xr = static_cast<int32_t>(mi * kPairRows + side * 128);
+      const int32_t wr = static_cast<int32_t>(ni * a.cols + side * half_cols);
+      for (int k = 0; k < count; ++k, ++i, p.next(a.stages)) {
+        if (i >= a.stages && !wait_or_abort(&empty[p.stage], p.phase ^ 1, &abort)) {
+          ok = false;
+          break;
         }
+        if (elect_one()) {
+          const uint32_t bar = bars + p.stage * 8;
+          // the first CTA's barrier counts the bytes of both
+          if (side == 0) mbar_expect_tx(&full[p.stage], 2 * stage_bytes);
+          uint8_t* dst = ring + p.stage * stage_bytes;
+          tma_load_pair(dst, &xmap, (s0 + k) * a.box_elems, xr, bar);
+          tma_load_pair(dst + xbytes, &wmap, (s0 + k) * a.box_elems, wr, bar);
+        }
+        __syncwarp();
       }
-      // every stage has landed and been read, and its barrier signalled, before the pair may exit
-      bool read = true;
-      for (int64_t j = i > a.stages ? i - a.stages : 0; j < i; ++j) {
-        read = read && wait_phase(&empty[j % a.stages], (j / a.stages) & 1);
-        if (!read && rank == 0) wait_phase(&full[j % a.stages], (j / a.stages) & 1);
-      }
+    }
+    // every stage has landed and been read, and its barrier signalled, before the pair may exit
+    bool read = true;
+    for (int64_t j = i > a.stages ? i - a.stages : 0; j < i; ++j) {
+      read = read && wait_phase(&empty[j % a.stages], (j / a.stages) & 1);
+      if (!read && side == 0) wait_phase(&full[j % a.stages], (j / a.stages) & 1);
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      RingPos p;
+    if (side == 0) {
+      const uint64_t ring_desc = tile_desc(smem_addr(ring));
+      RingPos p{0, 0};
       int it = 0;
       bool ok = true;
-      for (int64_t t = first; t < tiles && ok; t += pairs, ++it) {
+      for (int64_t t = first; t < tiles && ok; t += stride, ++it) {
         const int b = it & 1;
         if (!wait_or_abort(&acc_empty[b], ((it >> 1) & 1) ^ 1, &abort)) break;
         tc_fence_after();
         const uint32_t d = tmem + b * kPairCols;
-        for (int k = 0; k < a.steps; ++k, p.next(a.stages)) {
-          const int s = p.stage;
-          if (!wait_or_abort(&full[s], p.phase, &abort)) {
+        for (int k = 0; k < count;) {
+          const int here = wait_steps(full, p, a.stages, count - k, &abort);
+          if (here == 0) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint32_t x = smem_addr(ring + static_cast<size_t>(s) * stage_bytes), w = x + xbytes;
+          for (int j = 0; j < here; ++j, ++k, p.next(a.stages)) {
+            const uint64_t x = ring_desc + p.stage * (stage_bytes / 16), w = x + xbytes / 16;
+            if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < kBoxBytes; kk += kSliceBytes)
-            tc_mma<FP8, 2>(d, tile_desc(x + kk), tile_desc(w + kk), a.desc, k + kk > 0);
-          tc_commit<2>(&empty[s]);
+              for (int kk = 0; kk < kBoxBytes; kk += kSliceBytes)
+                tc_mma<FP8, 2>(d, x + kk / 16, w + kk / 16, a.desc, k + kk > 0);
+              tc_commit<2>(&empty[p.stage], both);
+              if (k + 1 == count) tc_commit<2>(&acc_full[b], both);
+            }
+            __syncwarp();
+          }
         }
-        if (ok) tc_commit<2>(&acc_full[b]);
       }
     }
     __syncwarp();
   } else if (warp >= 4) {
     const int q = warp - 4, et = threadIdx.x - 128;
-    float* stage = s_stage[q];
     int it = 0;
     bool ok = true;
-    for (int64_t t = first; t < tiles; t += pairs, ++it) {
+    for (int64_t t = first; t < tiles; t += stride, ++it) {
       const int b = it & 1;
       int64_t mi, ni;
       pair_tile(a, t, &mi, &ni);
-      const int64_t n0 = ni * a.cols, m0 = mi * kPairRows + rank * 128 + q * 32, m = m0 + lane;
+      const int64_t n0 = ni * a.cols, m0 = mi * kPairRows + side * 128 + q * 32, m = m0 + lane;
       // the tile's bias and weight scales, loaded under its MMAs
       for (int c = et; c < a.cols; c += 128) {
         const int64_t n = n0 + c;
@@ -653,64 +851,65 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const float xs = FP8 && m < a.e.m ? a.e.xs[m] : 1.f;
       named_sync(1, 128);
       // after an expired wait the four warps still meet at every tile's barrier
-      ok = __all_sync(0xffffffffu, ok && wait_or_abort(&acc_full[b], (it >> 1) & 1, &abort));
+      ok = ok && wait_or_abort(&acc_full[b], (it >> 1) & 1, &abort);
       if (!ok) continue;
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kPairCols;
+      if (a.split > 1) {
+        // the partial tile, a column of 128 rows after another, in the ring's memory
+        float* part = reinterpret_cast<float*>(ring) + q * 32 + lane;
+        for (int c = 0; c < a.cols; c += kChunk) {
+          uint32_t v[kChunk];
+          tc_load32(acc + c, v);
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) part[(c + j) * 128] = __uint_as_float(v[j]);
+        }
+        continue;
+      }
       for (int c = 0; c < a.cols; c += kChunk) {
         float v[kChunk];
         tc_load32(acc + c, reinterpret_cast<uint32_t*>(v));
         if (c + kChunk >= a.cols) {  // the accumulator is free for the tile after next
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive_cluster(cluster_map(&acc_empty[b], 0));
+          if (lane == 0) arrive_cluster(cluster_map(&acc_empty[b], crank - side));
         }
         if (n0 + c >= a.e.n || m0 >= a.e.m) continue;
-#pragma unroll
-        for (int j = 0; j < kChunk; ++j) {
-          if (FP8) v[j] = v[j] * xs * s_ws[b][c + j];
-          v[j] += s_bias[b][c + j];
-        }
-        activate_all<kChunk>(v, a.e.act);
-        if (a.vec) {
-          if (m < a.e.m) {
-            T* y = static_cast<T*>(a.e.y) + m * a.e.sym + n0 + c;
-            const T* ra = static_cast<const T*>(a.e.ra) + (a.e.ra ? m * a.e.srm + n0 + c : 0);
-#pragma unroll
-            for (int j = 0; j < kChunk; j += 8) {
-              if (n0 + c + j >= a.e.n) break;
-              if (a.e.ra) {
-                float f[8];
-                unpack8<T>(*reinterpret_cast<const uint4*>(ra + j), f);
-#pragma unroll
-                for (int u = 0; u < 8; ++u) v[j + u] += f[u];
-              }
-              *reinterpret_cast<uint4*>(y + j) = pack8<T>(v + j);
-            }
-          }
-        } else {
-          // any layout of y and row_add: through shared memory, a row of 32
-          // consecutive columns at a time
-          __syncwarp();
-#pragma unroll
-          for (int j = 0; j < kChunk; ++j) stage[lane * kStagePitch + j] = v[j];
-          __syncwarp();
-          const int64_t n = n0 + c + lane;
-          if (n < a.e.n) {
-            for (int r = 0; r < 32 && m0 + r < a.e.m; ++r) {
-              float o = stage[r * kStagePitch + lane];
-              if (a.e.ra) o += load_as_f32(a.e.ra, a.e.ra_dtype, (m0 + r) * a.e.srm + n * a.e.srn);
-              static_cast<T*>(a.e.y)[(m0 + r) * a.e.sym + n * a.e.syn] = from_f32<T>(o);
-            }
-          }
-        }
+        emit_chunk<T, FP8>(a, v, m0, n0 + c, xs, s_ws[b] + c, s_bias[b] + c, s_stage[q]);
       }
     }
     __syncwarp();
   }
+  if (a.split > 1) {
+    cluster_arrive();  // every partial is written
+    cluster_wait();
+    // all eight warps where y takes vectors, else the four with a staging buffer
+    if (a.vec || warp >= 4) {
+      const int q = warp & 3, turn = a.vec ? warp >> 2 : 0, turns = a.vec ? 2 : 1;
+      int64_t mi, ni;
+      pair_tile(a, first, &mi, &ni);
+      const int64_t n0 = ni * a.cols, m0 = mi * kPairRows + side * 128 + q * 32, m = m0 + lane;
+      const float xs = FP8 && m < a.e.m ? a.e.xs[m] : 1.f;
+      const float* part = reinterpret_cast<float*>(ring) + q * 32 + lane;
+      for (int c = (pair * turns + turn) * kChunk; c < a.cols && m0 < a.e.m && n0 + c < a.e.n;
+           c += a.split * turns * kChunk) {
+        float v[kChunk] = {};
+        for (int o = 0; o < a.split; ++o) {
+          const uint32_t from = cluster_map(part + c * 128, 2 * o + side);
+          float w[kChunk];  // all on their way before the first is added
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) w[j] = ld_cluster_f32(from + j * 512);
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j) v[j] += w[j];
+        }
+        emit_chunk<T, FP8>(a, v, m0, n0 + c, xs, s_ws[0] + c, s_bias[0] + c, s_stage[q]);
+      }
+      __syncwarp();
+    }
+  }
   tc_fence_before();
   __syncthreads();
-  cluster_arrive();  // the pair's last signals and MMAs have arrived on both sides
+  cluster_arrive();  // the cluster's last signals, MMAs and reads of partials are over on all sides
   cluster_wait();
   if (warp == 2) {
     tc_fence_after();
@@ -749,12 +948,44 @@ bool operand_map(CUtensorMap* map, const void* p, int64_t rows, int64_t k, int64
 }
 
 constexpr size_t kSmemMax = 227 * 1024;
-// Tensor memory has 512 columns an SM and an allocation waits for them.  A
-// split CTA takes at most 256 and at least this much shared memory, a pair CTA
-// all 512 and more than 228 KB less this: no SM ever holds CTAs of theirs that
-// want more than there is, so no allocation waits for a CTA that is itself
-// waiting for a peer.
-constexpr size_t kSplitSmemMin = 80 * 1024;
+// Tensor memory has 512 columns an SM and an allocation waits for them.  A CTA
+// takes at least this much shared memory for each column, its share of the
+// SM's 228 KB: no SM ever holds CTAs that want more columns than there are, so
+// no allocation waits for a CTA that is itself waiting for a peer.
+constexpr size_t kSmemPerTmemCol = 228 * 1024 / 512;
+
+// Clusters of `size` CTAs that fit on the device at once, one CTA per SM.
+template <typename Kern>
+int64_t cluster_slots(Kern kern, int size) {
+  static std::mutex mu;
+  static std::map<std::tuple<const void*, int, int>, int> known;
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  const auto key = std::make_tuple(reinterpret_cast<const void*>(kern), dev, size);
+  std::lock_guard<std::mutex> lock(mu);
+  auto it = known.find(key);
+  if (it != known.end()) return it->second;
+  const size_t smem = 200 * 1024;
+  int n = 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(size));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(size);
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess ||
+      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+    (void)cudaGetLastError();
+    n = 1;
+  }
+  known[key] = n;
+  return n;
+}
 
 template <typename Kern, typename Args>
 cudaError_t launch_cluster(Kern kern, dim3 grid, int threads, int cluster, size_t smem, cudaStream_t st,
@@ -780,58 +1011,74 @@ cudaError_t launch_cluster(Kern kern, dim3 grid, int threads, int cluster, size_
 
 int mma_format(int in_dtype) { return in_dtype == FD_BF16 ? 1 : 0; }
 
+// Rows of y (and of row_add, where there is one) as vectors of `width` elements of the output's type.
+bool epilogue_vec(const Epilogue& e, int out_dtype, int width) {
+  auto rows = [&](const void* p, int64_t stride) {
+    return reinterpret_cast<uintptr_t>(p) % (2 * width) == 0 && (e.m == 1 || stride % width == 0);
+  };
+  if (e.syn != 1 || !rows(e.y, e.sym)) return false;
+  return !e.ra || (e.ra_dtype == out_dtype && e.srn == 1 && rows(e.ra, e.srm));
+}
+
+// Rows of x up to which the split kernel serves a product.  Each of its CTAs
+// takes in (R + rows of x) * 128 bytes a step, so the pair kernel, which shares
+// the x tile between two CTAs, wins once x is no longer small beside R.  In 16
+// bits, split and pair at 64 / 96 / 128 rows: 4096 x 4096 12.1, 14.5 / 14.2,
+// 14.8 / 15.2, 15.2 us; 28672 x 4096 46.9, 53.3 / 60.3, 54.3 / 62.5, 55.1 us.
+constexpr int64_t kSplitMaxM = 80;
+
 // Few rows.  FD_ERR_UNSUPPORTED: a layout TMA cannot address.
 template <typename T, bool FP8>
-int launch_split(const GenericArgs& g, int in_dtype, bool w_early, cudaStream_t st) {
+int launch_split(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t st) {
   constexpr int es = FP8 ? 1 : 2;
+  constexpr int64_t max_rows = 256;
   const Epilogue& e = g.epi;
   SplitArgs a;
   a.e = e;
-  const int64_t mblocks = (e.m + 255) / 256;
-  const int64_t per = (e.m + mblocks - 1) / mblocks;
-  a.cols = static_cast<int32_t>((per + 15) / 16 * 16);
-  a.boxes = a.cols <= 64 ? 2 : 1;
+  a.cols = static_cast<int32_t>((e.m + 15) / 16 * 16);
   a.box_elems = kBoxBytes / es;
-  const int64_t steps = (g.k + a.boxes * a.box_elems - 1) / (a.boxes * a.box_elems);
-  const int64_t nblocks = (e.n + kTileRows - 1) / kTileRows;
-  const int64_t tiles = nblocks * mblocks;
   const int sms = fd_host::sm_count();
-  int split = 1;
-  while (split < kMaxSplit && tiles * split * 2 <= sms && steps >= split * 4) split *= 2;
-  if (const char* env = std::getenv("FD_PRODUCT_TUNE")) {
-    int b = 0, c = 0;
-    if (std::sscanf(env, "%d,%d", &b, &c) == 2) {
-      if (b > 0) a.boxes = b;
-      if (c > 0) split = c;
-    }
-  }
-  if (steps > 0x7fffffffLL || nblocks * split > 0x7fffffffLL || mblocks > 65535) return FD_ERR_UNSUPPORTED;
+  const int64_t steps = (g.k + a.box_elems - 1) / a.box_elems;
+  // CTAs per tile: tiles of about 128 rows (an MMA takes as long for fewer)
+  // that fill the SMs, 8 steps at least to each CTA
+  a.split = 1;
+  while (a.split < kMaxSplit && e.n * a.split * 2 <= static_cast<int64_t>(sms) * kBlockRows && steps >= a.split * 8)
+    a.split *= 2;
+  // R: equal tiles in one wave of CTAs, or in the fewest
+  const int64_t slots = a.split > 1 ? cluster_slots(product_split_kernel<T, FP8>, a.split) : sms;
+  const int64_t waves = a.split > 1 ? 1 : (e.n + slots * max_rows - 1) / (slots * max_rows);
+  const int64_t rows = std::min<int64_t>(((e.n + slots * waves - 1) / (slots * waves) + 7) / 8 * 8, max_rows);
+  a.rows = static_cast<int32_t>(rows);
+  a.blocks = a.rows > kBlockRows ? 2 : 1;
+  a.tiles = (e.n + rows - 1) / rows;
+  if (steps > 0x7fffffffLL || a.tiles > 0x7fffff) return FD_ERR_UNSUPPORTED;
   a.steps = static_cast<int32_t>(steps);
-  a.split = split;
-  a.desc = mma_desc(FP8 ? 0 : mma_format(in_dtype), kTileRows, a.cols);
+  a.desc = mma_desc(FP8 ? 0 : mma_format(in_dtype), kBlockRows, a.cols);
+  const uint32_t acc = a.blocks * a.cols;
+  a.accs = a.split == 1 && a.tiles > sms && 2 * acc <= 256 ? 2 : 1;
   a.tmem_cols = 32;
-  while (a.tmem_cols < static_cast<uint32_t>(a.cols)) a.tmem_cols *= 2;
-  a.w_early = w_early;
-  const size_t stage = static_cast<size_t>(a.boxes) * kBoxBytes * (kTileRows + a.cols);
-  const size_t part = split > 1 ? static_cast<size_t>(a.cols) * kTileRows * 4 : 0;
-  size_t budget = tiles * split > sms ? 110 * 1024 : 220 * 1024;
-  a.stages = static_cast<int32_t>(std::min<size_t>(kMaxRing, budget / stage));
-  if (a.stages < 2) a.stages = 2;
-  const size_t smem = std::max(kSplitSmemMin, std::max(a.stages * stage, part) + 1024);
+  while (a.tmem_cols < a.accs * acc) a.tmem_cols *= 2;
+  a.vec = epilogue_vec(e, out_dtype, 4);
+  // A ring of half the shared memory lets the next kernel's CTAs start beside
+  // this one's and bring their first tiles into L2; a long stream gains more
+  // from a ring of all of it (28672 x 4096 in 16 bits, 1.6 MB a CTA: 38.9
+  // against 40.1 us; 4096 x 14336 in 8 bits, 0.46 MB a CTA: 14.4 against 14.1).
+  const bool deep = steps / a.split * a.rows * kBoxBytes >= 768 * 1024;
+  a.ahead = deep ? 8 : 4;
+  const size_t stage = static_cast<size_t>(kBoxBytes) * (a.rows + a.cols);
+  a.stages = static_cast<int32_t>(std::min<size_t>(kMaxRing, (deep ? 216 : 108) * 1024 / stage));
+  const size_t part = a.split > 1 ? static_cast<size_t>(e.m) * a.rows * 4 : 0;
+  // an MMA reads whole blocks of 128 rows, past the last stage's R
+  const size_t reads = (a.stages - 1) * stage + static_cast<size_t>(kBoxBytes) * a.blocks * kBlockRows;
+  const size_t smem = std::max(a.tmem_cols * kSmemPerTmemCol, std::max(std::max(a.stages * stage, reads), part) + 1024);
   if (smem > kSmemMax - 1024) return FD_ERR_UNSUPPORTED;
   CUtensorMap wm, xm;
-  if (!operand_map(&wm, g.w, e.n, g.k, g.swn, g.swk, es, kTileRows) ||
+  if (!operand_map(&wm, g.w, e.n, g.k, g.swn, g.swk, es, a.rows) ||
       !operand_map(&xm, g.x, e.m, g.k, g.sxm, g.sxk, es, a.cols))
     return FD_ERR_UNSUPPORTED;
-  const dim3 grid(static_cast<unsigned>(nblocks * split), static_cast<unsigned>(mblocks));
-  return from_cuda(launch_cluster(product_split_kernel<T, FP8>, grid, kSplitThreads, split, smem, st, wm, xm, a));
-}
-
-// Rows of y (and of row_add, where there is one) as vectors of 8 of type T.
-bool epilogue_vec(const Epilogue& e, int out_dtype) {
-  if (e.n % 8 || e.syn != 1 || e.sym % 8 || !fd_host::aligned16(e.y)) return false;
-  if (!e.ra) return true;
-  return e.ra_dtype == out_dtype && e.srn == 1 && e.srm % 8 == 0 && fd_host::aligned16(e.ra);
+  const int64_t grid = a.split > 1 ? a.tiles * a.split : std::min<int64_t>(a.tiles, sms);
+  return from_cuda(launch_cluster(product_split_kernel<T, FP8>, dim3(static_cast<unsigned>(grid)), kSplitThreads,
+                                  a.split, smem, st, wm, xm, a));
 }
 
 template <typename T, bool FP8>
@@ -844,50 +1091,53 @@ int launch_pair(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t 
   const int64_t steps = (g.k + a.box_elems - 1) / a.box_elems;
   const int pairs = fd_host::sm_count() / 2;
   a.mt = (e.m + kPairRows - 1) / kPairRows;
-  // columns per tile: the widest that wastes least of the last wave
-  int64_t best = 0;
+  // Columns per tile and pairs per tile, by the time they should take: a step
+  // measured 0.12 us + 0.98 ns per column (0.245 at 128 columns, 0.37 at 256,
+  // MMAs, L2 and the power limit together), a tile's start and end 0.5 us, the
+  // exchange of partials 0.5 us + 6 ns per column.
+  double best = 0;
   a.cols = 0;
-  for (int c = kPairCols; c >= 128; c -= 32) {
-    const int64_t tiles = a.mt * ((e.n + c - 1) / c);
-    const int64_t cost = (tiles + pairs - 1) / pairs * (c + 16);
-    if (a.cols == 0 || cost < best) {
-      best = cost;
-      a.cols = c;
+  a.split = 1;
+  for (int split = 1; split <= 4 && (split == 1 || steps >= 4 * split); split *= 2) {
+    const int64_t slots = split > 1 ? cluster_slots(product_pair_kernel<T, FP8>, 2 * split) : pairs;
+    for (int c = kPairCols; c >= 64; c -= kChunk) {
+      const int64_t tiles = a.mt * ((e.n + c - 1) / c);
+      const int64_t waves = (tiles + slots - 1) / slots;
+      if (split > 1 && waves > 1) continue;
+      const double cost = waves * ((steps + split - 1) / split * (0.12 + 0.00098 * c) + 0.5) +
+                          (split > 1 ? 0.5 + 0.006 * c : 0.0);
+      if (a.cols == 0 || cost < best) {
+        best = cost;
+        a.cols = c;
+        a.split = split;
+      }
     }
   }
-  a.group = 8;
-  int max_stages = kMaxRing;
-  if (const char* env = std::getenv("FD_PAIR_TUNE")) {
-    int b = 0, c = 0, d = 0;
-    if (std::sscanf(env, "%d,%d,%d", &b, &c, &d) == 3) {
-      if (b > 0) a.cols = b;
-      if (c > 0) a.group = c;
-      if (d > 0) max_stages = d;
-    }
-  }
+  a.group = 16;
   a.nt = (e.n + a.cols - 1) / a.cols;
   if (steps > 0x7fffffffLL || e.m > 0x7fffff00LL || e.n > 0x7fffff00LL) return FD_ERR_UNSUPPORTED;
   a.steps = static_cast<int32_t>(steps);
   a.desc = mma_desc(FP8 ? 0 : mma_format(in_dtype), kPairRows, a.cols);
-  a.vec = epilogue_vec(e, out_dtype);
+  a.vec = e.n % 8 == 0 && epilogue_vec(e, out_dtype, 8);
   const size_t stage = static_cast<size_t>(kBoxBytes) * (128 + a.cols / 2);
-  a.stages = static_cast<int32_t>(std::min<size_t>(max_stages, 192 * 1024 / stage));
-  const size_t smem = a.stages * stage + 1024;
+  a.stages = static_cast<int32_t>(std::min<size_t>(kMaxRing, 192 * 1024 / stage));
+  // all of an SM's shared memory, as all of its tensor memory
+  const size_t smem = std::max<size_t>(a.stages * stage + 1024, 204 * 1024);
   CUtensorMap xm, wm;
   if (!operand_map(&xm, g.x, e.m, g.k, g.sxm, g.sxk, es, 128) ||
       !operand_map(&wm, g.w, e.n, g.k, g.swn, g.swk, es, a.cols / 2))
     return FD_ERR_UNSUPPORTED;
-  const int64_t grid = 2 * std::min<int64_t>(pairs, a.mt * a.nt);
-  return from_cuda(launch_cluster(product_pair_kernel<T, FP8>, dim3(static_cast<unsigned>(grid)), kPairThreads, 2, smem,
-                                  st, xm, wm, a));
+  const int64_t grid = 2 * a.split * (a.split > 1 ? a.mt * a.nt : std::min<int64_t>(pairs, a.mt * a.nt));
+  return from_cuda(launch_cluster(product_pair_kernel<T, FP8>, dim3(static_cast<unsigned>(grid)), kPairThreads,
+                                  2 * a.split, smem, st, xm, wm, a));
 }
 
 template <typename TX, typename T, bool FP8>
-int launch_product(const GenericArgs& g, int in_dtype, int out_dtype, bool w_early, cudaStream_t st) {
+int launch_product(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t st) {
   int r = FD_ERR_UNSUPPORTED;
   if (g.k > 0) {
-    if (g.epi.m > 256) r = launch_pair<T, FP8>(g, in_dtype, out_dtype, st);
-    else r = launch_split<T, FP8>(g, in_dtype, w_early, st);
+    r = g.epi.m <= kSplitMaxM ? launch_split<T, FP8>(g, in_dtype, out_dtype, st)
+                              : launch_pair<T, FP8>(g, in_dtype, out_dtype, st);
   }
   return r == FD_ERR_UNSUPPORTED ? launch_generic<TX, T, FP8>(g, st) : r;
 }
@@ -898,20 +1148,18 @@ bool epilogue_ok(const Epilogue& e) {
 }
 
 // in_dtype: f16, bf16 or e4m3 (then e.xs and e.ws are set and out_dtype is the
-// output's; for 16-bit operands out_dtype = in_dtype).  w_early: the kernel
-// before this one on the stream does not write w, and has itself waited for
-// everything before it.
-int product(const GenericArgs& a, int in_dtype, int out_dtype, bool w_early, cudaStream_t st) {
+// output's; for 16-bit operands out_dtype = in_dtype).
+int product(const GenericArgs& a, int in_dtype, int out_dtype, cudaStream_t st) {
   const Epilogue& e = a.epi;
   if (e.m < 0 || e.n < 0 || a.k < 0) return FD_ERR_ARG;
   if (e.m == 0 || e.n == 0) return FD_OK;
   if (!epilogue_ok(e) || !fd_host::half_dtype(out_dtype) || (a.k > 0 && (!a.x || !a.w))) return FD_ERR_ARG;
   const bool bf = out_dtype == FD_BF16;
   if (in_dtype == FD_E4M3)
-    return bf ? launch_product<__half, __nv_bfloat16, true>(a, in_dtype, out_dtype, w_early, st)
-              : launch_product<__half, __half, true>(a, in_dtype, out_dtype, w_early, st);
-  return bf ? launch_product<__nv_bfloat16, __nv_bfloat16, false>(a, in_dtype, out_dtype, w_early, st)
-            : launch_product<__half, __half, false>(a, in_dtype, out_dtype, w_early, st);
+    return bf ? launch_product<__half, __nv_bfloat16, true>(a, in_dtype, out_dtype, st)
+              : launch_product<__half, __half, true>(a, in_dtype, out_dtype, st);
+  return bf ? launch_product<__nv_bfloat16, __nv_bfloat16, false>(a, in_dtype, out_dtype, st)
+            : launch_product<__half, __half, false>(a, in_dtype, out_dtype, st);
 }
 
 // ---- post_attn_mlp_fp8's intermediates in the caller's workspace
@@ -941,7 +1189,7 @@ int fd_linear_act_out(const void* x, int64_t sxm, int64_t sxk, const void* w, in
                       int64_t m, int64_t n, int64_t k, void* stream) {
   if (!fd_host::half_dtype(dtype)) return FD_ERR_ARG;
   const Epilogue e{nullptr, nullptr, bias, bias_dtype, sbias, row_add, ra_dtype, srm, srn, y, sym, syn, m, n, act};
-  return product({x, sxm, sxk, w, swn, swk, k, e}, dtype, dtype, false, static_cast<cudaStream_t>(stream));
+  return product({x, sxm, sxk, w, swn, swk, k, e}, dtype, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int fd_linear_fp8_out(const void* x, int64_t sxm, int64_t sxk, const float* x_scale, const void* w, int64_t swn,
@@ -950,7 +1198,7 @@ int fd_linear_fp8_out(const void* x, int64_t sxm, int64_t sxk, const float* x_sc
                       int64_t syn, int32_t out_dtype, int32_t act, int64_t m, int64_t n, int64_t k, void* stream) {
   if (m > 0 && n > 0 && (!x_scale || !w_scale)) return FD_ERR_ARG;
   const Epilogue e{x_scale, w_scale, bias, bias_dtype, sbias, row_add, ra_dtype, srm, srn, y, sym, syn, m, n, act};
-  return product({x, sxm, sxk, w, swn, swk, k, e}, FD_E4M3, out_dtype, false, static_cast<cudaStream_t>(stream));
+  return product({x, sxm, sxk, w, swn, swk, k, e}, FD_E4M3, out_dtype, static_cast<cudaStream_t>(stream));
 }
 
 int fd_product_status(int32_t* status, void* stream) {
