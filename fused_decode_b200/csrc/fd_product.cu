@@ -10,6 +10,7 @@
 #include <map>
 #include <mutex>
 #include <tuple>
+#include <type_traits>
 
 using namespace fd;
 
@@ -32,6 +33,11 @@ struct Epilogue {
   int64_t m, n;
   int32_t act;
 };
+
+template <typename T>
+FD_DEV constexpr int dtype_of() {
+  return std::is_same<T, __nv_bfloat16>::value ? FD_BF16 : FD_F16;
+}
 
 // v * sigmoid(z), with exp(-|z|) so that nothing overflows (see silu_mul for
 // the accuracy of __expf and __fdividef).
@@ -272,11 +278,6 @@ FD_DEV void tma_prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
 
 FD_DEV void bar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 FD_DEV void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-FD_DEV float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
 FD_DEV float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -368,6 +369,90 @@ FD_DEV void activate_all(float* v, int act) {
   }
 }
 
+constexpr int kMaxSplit = 8;  // CTAs, or pairs, that share a tile's K steps
+
+// Four consecutive columns of y from their sums.
+template <typename T, bool FP8>
+FD_DEV void finish4(const Epilogue& e, bool vec, int64_t m, int64_t n, const float* sum) {
+  if (!vec || n + 4 > e.n) {
+    for (int j = 0; j < 4 && n + j < e.n; ++j) finish<T, FP8>(e, m, n + j, sum[j]);
+    return;
+  }
+  float v[4];
+  const float xs = FP8 ? e.xs[m] : 1.f;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j] = FP8 ? sum[j] * xs * e.ws[n + j] : sum[j];
+    if (e.bias) v[j] += load_as_f32(e.bias, e.bias_dtype, (n + j) * e.sbias);
+  }
+  activate_all<4>(v, e.act);
+  if (e.ra) {
+    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const T*>(e.ra) + m * e.srm + n);
+    const float2 lo = unpack2<T>(w.x), hi = unpack2<T>(w.y);
+    v[0] += lo.x; v[1] += lo.y; v[2] += hi.x; v[3] += hi.y;
+  }
+  *reinterpret_cast<uint2*>(static_cast<T*>(e.y) + m * e.sym + n) =
+      make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+}
+
+// The partial tiles of a cluster's `parts` sharers, `rows` floats to a column
+// at `part` in each: sharer `rank` takes the columns rank, rank + parts, ... below
+// `live`, sums them in sharer order and finishes them, `threads` threads at
+// work.  Sharer p is the cluster's CTA p * step + side.
+template <typename T, bool FP8>
+FD_DEV void join_parts(const Epilogue& e, bool vec, const float* part, int rows, int live, int rank, int parts, int step,
+                       int side, int64_t m0, int64_t n0, int tid, int threads) {
+  const int quads = rows / 4, mine = live > rank ? (live - rank - 1) / parts + 1 : 0;
+  for (int i = tid; i < mine * quads; i += threads) {
+    const int c = rank + i / quads * parts, r = i % quads * 4;
+    float4 from[kMaxSplit];  // all on their way before the first is added
+#pragma unroll
+    for (int p = 0; p < kMaxSplit; ++p)
+      from[p] = p < parts ? ld_cluster_f4(fd_stream::cluster_map(part + c * rows + r, p * step + side))
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int p = 0; p < kMaxSplit; ++p) {
+      v[0] += from[p].x; v[1] += from[p].y; v[2] += from[p].z; v[3] += from[p].w;
+    }
+    if (n0 + r < e.n) finish4<T, FP8>(e, vec, m0 + c, n0 + r, v);
+  }
+}
+
+// N columns of a tile straight from tensor memory, `live` of them in use, one
+// row n of w to a thread: consecutive lanes write consecutive elements of y,
+// whatever its layout.  xs: the scales of the N rows of x.  The columns' offsets
+// from the first are 32-bit (the host keeps 32 row strides of y and row_add
+// below 2^32 elements).
+template <typename T, bool FP8, int N>
+FD_DEV void emit_columns(const Epilogue& e, float* v, int64_t m, int live, int64_t n, const float* xs, float ws,
+                         float bias) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) v[j] = FP8 ? fmaf(v[j] * xs[j], ws, bias) : v[j] + bias;
+  activate_all<N>(v, e.act);
+  const uint32_t sym = static_cast<uint32_t>(e.sym), srm = static_cast<uint32_t>(e.srm);
+  T* y = static_cast<T*>(e.y) + m * e.sym + n * e.syn;
+  if (live >= N && (!e.ra || e.ra_dtype == dtype_of<T>())) {
+    if (e.ra) {  // all on their way before the first is added
+      const T* ra = static_cast<const T*>(e.ra) + m * e.srm + n * e.srn;
+      T r[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) r[j] = ra[j * srm];
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] += to_f32(r[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) y[j * sym] = from_f32<T>(v[j]);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    if (j < live) {
+      if (e.ra) v[j] += load_as_f32(e.ra, e.ra_dtype, (m + j) * e.srm + n * e.srn);
+      y[j * sym] = from_f32<T>(v[j]);
+    }
+}
+
 // ============================================================== few rows
 // Products bound by the weight's bytes.  The weight's rows are cut into tiles
 // of R rows (any multiple of 8 up to 256) so that the tiles, or the tiles times
@@ -383,7 +468,6 @@ FD_DEV void activate_all(float* v, int act) {
 // more than SMs, the epilogue of one under the stream of the next.
 constexpr int kBlockRows = 128;  // rows of one MMA
 constexpr int kSplitThreads = 256;
-constexpr int kMaxSplit = 8;
 
 struct SplitArgs {
   Epilogue e;
@@ -401,30 +485,6 @@ struct SplitArgs {
   int32_t ahead;   // steps of w brought into L2 before the kernel before this one has finished
   int32_t vec;     // y and row_add take 4 columns at a time
 };
-
-// Four consecutive columns of y from their sums.
-template <typename T, bool FP8>
-FD_DEV void finish4(const SplitArgs& a, int64_t m, int64_t n, const float* sum) {
-  if (!a.vec || n + 4 > a.e.n) {
-    for (int j = 0; j < 4 && n + j < a.e.n; ++j) finish<T, FP8>(a.e, m, n + j, sum[j]);
-    return;
-  }
-  float v[4];
-  const float xs = FP8 ? a.e.xs[m] : 1.f;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    v[j] = FP8 ? sum[j] * xs * a.e.ws[n + j] : sum[j];
-    if (a.e.bias) v[j] += load_as_f32(a.e.bias, a.e.bias_dtype, (n + j) * a.e.sbias);
-  }
-  activate_all<4>(v, a.e.act);
-  if (a.e.ra) {
-    const uint2 w = *reinterpret_cast<const uint2*>(static_cast<const T*>(a.e.ra) + m * a.e.srm + n);
-    const float2 lo = unpack2<T>(w.x), hi = unpack2<T>(w.y);
-    v[0] += lo.x; v[1] += lo.y; v[2] += hi.x; v[3] += hi.y;
-  }
-  *reinterpret_cast<uint2*>(static_cast<T*>(a.e.y) + m * a.e.sym + n) =
-      make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-}
 
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(kSplitThreads, 1)
@@ -552,20 +612,14 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
           const float bias = a.e.bias && row_ok ? load_as_f32(a.e.bias, a.e.bias_dtype, n * a.e.sbias) : 0.f;
           const uint32_t acc = tmem + (static_cast<uint32_t>((warp - 4) * 32) << 16) + b * acc_cols + blk * a.cols;
           for (int c = 0; c < live; c += 16) {
-            float v[16];
+            float v[16], xs[16];
             tc_load16(acc + c, reinterpret_cast<uint32_t*>(v));
             if (!row_ok) continue;
+            if (FP8) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              v[j] = (FP8 ? v[j] * (c + j < live ? a.e.xs[c + j] : 0.f) * ws : v[j]) + bias;
-            activate_all<16>(v, a.e.act);
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int64_t m = c + j;
-              if (m >= live) break;
-              if (a.e.ra) v[j] += load_as_f32(a.e.ra, a.e.ra_dtype, m * a.e.srm + n * a.e.srn);
-              static_cast<T*>(a.e.y)[m * a.e.sym + n * a.e.syn] = from_f32<T>(v[j]);
+              for (int j = 0; j < 16; ++j) xs[j] = c + j < live ? a.e.xs[c + j] : 0.f;
             }
+            emit_columns<T, FP8, 16>(a.e, v, c, live - c, n, xs, ws, bias);
           }
           __syncwarp();
         }
@@ -598,24 +652,13 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     __syncwarp();
     cluster_arrive();
     cluster_wait();
-    const int quads = a.rows / 4;
-    const int mine = live > static_cast<int>(rank) ? (live - static_cast<int>(rank) - 1) / a.split + 1 : 0;  // columns
-    for (int i = threadIdx.x; i < mine * quads; i += kSplitThreads) {
-      const int c = static_cast<int>(rank) + i / quads * a.split, r = i % quads * 4;
-      float4 from[kMaxSplit];  // all on their way before the first is added
-#pragma unroll
-      for (int p = 0; p < kMaxSplit; ++p)
-        from[p] = p < a.split ? ld_cluster_f4(cluster_map(part + c * a.rows + r, p)) : make_float4(0.f, 0.f, 0.f, 0.f);
-      float v[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int p = 0; p < kMaxSplit; ++p) {
-        v[0] += from[p].x; v[1] += from[p].y; v[2] += from[p].z; v[3] += from[p].w;
-      }
-      const int64_t n = first * a.rows + r;
-      if (n < a.e.n) finish4<T, FP8>(a, c, n, v);
-    }
+    join_parts<T, FP8>(a.e, a.vec, part, a.rows, live, rank, a.split, 1, 0, 0, first * a.rows, threadIdx.x,
+                       kSplitThreads);
     __syncwarp();
-    cluster_arrive();  // the other CTAs may still be reading this one's partial
+    // The other CTAs may still be reading this one's partial.  Relaxed, here and
+    // in the pair kernel: nothing is passed on, and a release would wait for
+    // this CTA's stores to y.
+    cluster_arrive_relaxed();
     cluster_wait();
   }
   __syncwarp();
@@ -628,38 +671,45 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 }
 
 // ============================================================== many rows
-// Pairs of CTAs (cta_group::2) on tiles of 256 rows of x by up to 256 rows of
-// w: each CTA holds 128 rows of the x tile and half of the w tile, so a pair
-// reads every operand byte from shared memory half as often as two single
-// CTAs would.  Persistent: a pair walks over its tiles with two accumulators
-// in tensor memory, the epilogue of one tile under the MMAs of the next.
+// Pairs of CTAs (cta_group::2) on tiles of 256 rows of w by up to 256 rows of x
+// (any multiple of 32, so that a ragged batch fills its tiles): each CTA holds
+// 128 rows of the w tile and half of the x tile, so a pair reads every operand
+// byte from shared memory half as often as two single CTAs would.  Persistent:
+// a pair walks over its tiles with two accumulators in tensor memory, the
+// epilogue of one tile under the MMAs of the next.  Rows of w are the MMA's rows
+// because the accumulator then has consecutive elements of a row of y in
+// consecutive lanes: one path of coalesced stores for any layout of y.
+// An SM takes in about 115 GB/s from L2 whatever it multiplies; where there are
+// fewer tiles than pairs, the pairs of a cluster share the K steps of one tile,
+// and each sums its part of the columns over all partials, in rank order,
+// through distributed shared memory.
 constexpr int kPairRows = 256;
-constexpr int kPairCols = 256;  // at most; a multiple of 32
-constexpr int kPairThreads = 256;
-constexpr int kChunk = 32;      // accumulator columns an epilogue warp handles at once
-constexpr int kStagePitch = kChunk + 1;
+constexpr int kPairCols = 256;     // at most
+constexpr int kPairThreads = 384;  // TMA, MMA, tensor memory, idle; eight epilogue warps
+constexpr int kChunk = 32;         // accumulator columns an epilogue warp handles at once
 
 struct PairArgs {
   Epilogue e;
   int32_t steps;  // 128-byte boxes along K
-  int32_t cols;   // rows of w per tile
+  int32_t cols;   // rows of x per tile
   int32_t stages;
   int32_t split;  // pairs that share a tile
   int32_t box_elems;
   uint32_t desc;
-  int64_t mt, nt;  // tiles along m and n
+  int64_t mt, nt;  // tiles along m (x) and n (w)
   int32_t group;   // m tiles walked together
-  int32_t vec;     // y and row_add rows are vectors of 8
+  int32_t vec;     // y and row_add take 4 columns at a time
 };
 
 // Tile t of the walk: `group` m tiles side by side for every n tile, so that
 // the pairs at work share both operands' tiles in L2.
 FD_DEV void pair_tile(const PairArgs& a, int64_t t, int64_t* mi, int64_t* ni) {
-  const int64_t per = static_cast<int64_t>(a.group) * a.nt;
-  const int64_t g = t / per, in = t % per;
-  const int64_t rows = min(static_cast<int64_t>(a.group), a.mt - g * a.group);
-  *mi = g * a.group + in % rows;
-  *ni = in / rows;
+  const uint32_t per = static_cast<uint32_t>(a.group) * static_cast<uint32_t>(a.nt), tile = static_cast<uint32_t>(t);
+  const uint32_t g = tile / per, in = tile - g * per;
+  const uint32_t rows = min(static_cast<uint32_t>(a.group), static_cast<uint32_t>(a.mt) - g * a.group);
+  const uint32_t n = in / rows;
+  *mi = g * a.group + (in - n * rows);
+  *ni = n;
 }
 
 FD_DEV void tma_load_pair(void* dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
@@ -669,73 +719,29 @@ FD_DEV void tma_load_pair(void* dst, const CUtensorMap* map, int32_t x, int32_t 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// Relaxed: the accumulator's columns are in registers by then, and a release
+// would wait for the warp's stores to y (about 2 us a tile).
 FD_DEV void arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-
-// Columns c .. c + 31 of 32 rows of a tile, from their sums: lane l holds row m0 + l.
-template <typename T, bool FP8>
-FD_DEV void emit_chunk(const PairArgs& a, float* v, int64_t m0, int64_t n0, float xs, const float* ws, const float* bias,
-                       float* stage) {
-  const int lane = threadIdx.x & 31;
-  const int64_t m = m0 + lane;
-#pragma unroll
-  for (int j = 0; j < kChunk; ++j) {
-    if (FP8) v[j] = v[j] * xs * ws[j];
-    v[j] += bias[j];
-  }
-  activate_all<kChunk>(v, a.e.act);
-  if (a.vec) {
-    if (m >= a.e.m) return;
-    T* y = static_cast<T*>(a.e.y) + m * a.e.sym + n0;
-    const T* ra = static_cast<const T*>(a.e.ra) + (a.e.ra ? m * a.e.srm + n0 : 0);
-#pragma unroll
-    for (int j = 0; j < kChunk; j += 8) {
-      if (n0 + j >= a.e.n) break;
-      if (a.e.ra) {
-        float f[8];
-        unpack8<T>(*reinterpret_cast<const uint4*>(ra + j), f);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) v[j + u] += f[u];
-      }
-      *reinterpret_cast<uint4*>(y + j) = pack8<T>(v + j);
-    }
-    return;
-  }
-  // any layout of y and row_add: through shared memory, a row of 32
-  // consecutive columns at a time
-  __syncwarp();
-#pragma unroll
-  for (int j = 0; j < kChunk; ++j) stage[lane * kStagePitch + j] = v[j];
-  __syncwarp();
-  const int64_t n = n0 + lane;
-  if (n < a.e.n) {
-    for (int r = 0; r < 32 && m0 + r < a.e.m; ++r) {
-      float o = stage[r * kStagePitch + lane];
-      if (a.e.ra) o += load_as_f32(a.e.ra, a.e.ra_dtype, (m0 + r) * a.e.srm + n * a.e.srn);
-      static_cast<T*>(a.e.y)[(m0 + r) * a.e.sym + n * a.e.syn] = from_f32<T>(o);
-    }
-  }
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 
 template <typename T, bool FP8>
 __global__ void __launch_bounds__(kPairThreads, 1)
-    product_pair_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+    product_pair_kernel(const __grid_constant__ CUtensorMap wmap, const __grid_constant__ CUtensorMap xmap,
                         const __grid_constant__ PairArgs a) {
   using namespace fd_stream;
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t full[kMaxRing], empty[kMaxRing], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort;
-  __shared__ __align__(16) float s_bias[2][kPairCols], s_ws[2][kPairCols];
-  __shared__ float s_stage[4][32 * kStagePitch];
+  __shared__ __align__(16) float s_xs[2][kPairCols];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t{1023});
   const int warp = warp_index(), lane = threadIdx.x & 31;
   // a cluster's CTAs: pairs of neighbours, the first of a pair issues its MMAs
   const uint32_t crank = cluster_ctarank(), side = crank & 1, pair = crank >> 1;
   const uint16_t both = static_cast<uint16_t>(3u << (pair * 2));
   const int half_cols = a.cols / 2;
-  const uint32_t xbytes = 128 * kBoxBytes, wbytes = half_cols * kBoxBytes, stage_bytes = xbytes + wbytes;
+  const uint32_t wbytes = 128 * kBoxBytes, xbytes = half_cols * kBoxBytes, stage_bytes = wbytes + xbytes;
   const int64_t tiles = a.mt * a.nt, stride = gridDim.x / (2 * a.split), first = blockIdx.x / (2 * a.split);
   const int s0 = static_cast<int>(static_cast<int64_t>(pair) * a.steps / a.split);
   const int count = static_cast<int>(static_cast<int64_t>(pair + 1) * a.steps / a.split) - s0;
@@ -747,7 +753,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 8);  // four epilogue warps of each CTA
+      mbar_init(&acc_empty[b], 16);  // eight epilogue warps of each CTA
     }
     abort = 0;
     bar_init_fence();
@@ -755,7 +761,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   if (warp == 2) tmem_alloc<2>(&tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
-  cluster_arrive();  // both CTAs' barriers exist before either is signalled
+  cluster_arrive_relaxed();  // the cluster's barriers exist (bar_init_fence) before any is signalled
   cluster_wait();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
@@ -764,8 +770,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
 
   if (warp == 0) {
     if (elect_one()) {
-      prefetch_map(&xmap);
       prefetch_map(&wmap);
+      prefetch_map(&xmap);
     }
     const uint32_t bars = cluster_map(full, crank - side);
     RingPos p{0, 0};
@@ -774,8 +780,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     for (int64_t t = first; t < tiles && ok; t += stride) {
       int64_t mi, ni;
       pair_tile(a, t, &mi, &ni);
-      const int32_t xr = static_cast<int32_t>(mi * kPairRows + side * 128);
-      const int32_t wr = static_cast<int32_t>(ni * a.cols + side * half_cols);
+      const int32_t wr = static_cast<int32_t>(ni * kPairRows + side * 128);
+      const int32_t xr = static_cast<int32_t>(mi * a.cols + side * half_cols);
       for (int k = 0; k < count; ++k, ++i, p.next(a.stages)) {
         if (i >= a.stages && !wait_or_abort(&empty[p.stage], p.phase ^ 1, &abort)) {
           ok = false;
@@ -786,8 +792,8 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           // the first CTA's barrier counts the bytes of both
           if (side == 0) mbar_expect_tx(&full[p.stage], 2 * stage_bytes);
           uint8_t* dst = ring + p.stage * stage_bytes;
-          tma_load_pair(dst, &xmap, (s0 + k) * a.box_elems, xr, bar);
-          tma_load_pair(dst + xbytes, &wmap, (s0 + k) * a.box_elems, wr, bar);
+          tma_load_pair(dst, &wmap, (s0 + k) * a.box_elems, wr, bar);
+          tma_load_pair(dst + wbytes, &xmap, (s0 + k) * a.box_elems, xr, bar);
         }
         __syncwarp();
       }
@@ -818,11 +824,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
           }
           tc_fence_after();
           for (int j = 0; j < here; ++j, ++k, p.next(a.stages)) {
-            const uint64_t x = ring_desc + p.stage * (stage_bytes / 16), w = x + xbytes / 16;
+            const uint64_t w = ring_desc + p.stage * (stage_bytes / 16), x = w + wbytes / 16;
             if (elect_one()) {
 #pragma unroll
               for (int kk = 0; kk < kBoxBytes; kk += kSliceBytes)
-                tc_mma<FP8, 2>(d, x + kk / 16, w + kk / 16, a.desc, k + kk > 0);
+                tc_mma<FP8, 2>(d, w + kk / 16, x + kk / 16, a.desc, k + kk > 0);
               tc_commit<2>(&empty[p.stage], both);
               if (k + 1 == count) tc_commit<2>(&acc_full[b], both);
             }
@@ -833,83 +839,87 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     __syncwarp();
   } else if (warp >= 4) {
-    const int q = warp - 4, et = threadIdx.x - 128;
-    int it = 0;
-    bool ok = true;
-    for (int64_t t = first; t < tiles; t += stride, ++it) {
-      const int b = it & 1;
+    const int q = warp & 3, turn = (warp - 4) >> 2, et = threadIdx.x - 128;
+    // a tile's place, this thread's scales (of row n of w, and of the tile's row
+    // et of x) and bias: loaded a tile ahead
+    struct Edge {
+      int64_t m0, n;
+      int live;
+      float ws, bias, xs;
+    };
+    auto edge_of = [&](int64_t t) {
+      Edge g{0, 0, 0, 1.f, 0.f, 0.f};
+      if (t >= tiles) return g;
       int64_t mi, ni;
       pair_tile(a, t, &mi, &ni);
-      const int64_t n0 = ni * a.cols, m0 = mi * kPairRows + side * 128 + q * 32, m = m0 + lane;
-      // the tile's bias and weight scales, loaded under its MMAs
-      for (int c = et; c < a.cols; c += 128) {
-        const int64_t n = n0 + c;
-        const bool in = n < a.e.n;
-        s_bias[b][c] = a.e.bias && in ? load_as_f32(a.e.bias, a.e.bias_dtype, n * a.e.sbias) : 0.f;
-        if (FP8) s_ws[b][c] = in ? a.e.ws[n] : 0.f;
+      g.m0 = mi * a.cols;
+      g.n = ni * kPairRows + side * 128 + q * 32 + lane;
+      g.live = static_cast<int>(min(static_cast<int64_t>(a.cols), a.e.m - g.m0));
+      if (g.n < a.e.n) {
+        if (FP8) g.ws = a.e.ws[g.n];
+        if (a.e.bias) g.bias = load_as_f32(a.e.bias, a.e.bias_dtype, g.n * a.e.sbias);
       }
-      const float xs = FP8 && m < a.e.m ? a.e.xs[m] : 1.f;
-      named_sync(1, 128);
-      // after an expired wait the four warps still meet at every tile's barrier
+      if (FP8 && et < g.live) g.xs = a.e.xs[g.m0 + et];
+      return g;
+    };
+    static_assert(kPairCols == kPairThreads - 128, "one row of x to a thread");
+    int it = 0;
+    bool ok = true;
+    Edge next = edge_of(first);
+    for (int64_t t = first; t < tiles; t += stride, ++it) {
+      const int b = it & 1;
+      const Edge g = next;
+      const int64_t m0 = g.m0, n = g.n;
+      const int live = g.live;
+      const bool row_ok = n < a.e.n;
+      if (FP8) {
+        s_xs[b][et] = g.xs;
+        named_sync(1, 256);
+      }
+      next = edge_of(t + stride);
+      // after an expired wait the eight warps still meet at every tile's barrier
       ok = ok && wait_or_abort(&acc_full[b], (it >> 1) & 1, &abort);
       if (!ok) continue;
       tc_fence_after();
       const uint32_t acc = tmem + (static_cast<uint32_t>(q * 32) << 16) + b * kPairCols;
-      if (a.split > 1) {
-        // the partial tile, a column of 128 rows after another, in the ring's memory
-        float* part = reinterpret_cast<float*>(ring) + q * 32 + lane;
-        for (int c = 0; c < a.cols; c += kChunk) {
-          uint32_t v[kChunk];
-          tc_load32(acc + c, v);
-#pragma unroll
-          for (int j = 0; j < kChunk; ++j) part[(c + j) * 128] = __uint_as_float(v[j]);
-        }
-        continue;
-      }
-      for (int c = 0; c < a.cols; c += kChunk) {
+      // the partial tile of a shared one: a column of 128 rows after another, in the ring's memory
+      float* part = reinterpret_cast<float*>(ring) + q * 32 + lane;
+      auto freed = [&]() {  // this warp has read its part: once from all, the accumulator takes the tile after next
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(cluster_map(&acc_empty[b], crank - side));
+      };
+      for (int c = turn * kChunk; c < live; c += 2 * kChunk) {
         float v[kChunk];
         tc_load32(acc + c, reinterpret_cast<uint32_t*>(v));
-        if (c + kChunk >= a.cols) {  // the accumulator is free for the tile after next
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) arrive_cluster(cluster_map(&acc_empty[b], crank - side));
+        if (c + 2 * kChunk >= live) freed();
+        if (a.split > 1) {
+#pragma unroll
+          for (int j = 0; j < kChunk; ++j)
+            if (c + j < live) part[(c + j) * 128] = v[j];
+        } else if (row_ok) {
+          emit_columns<T, FP8, kChunk>(a.e, v, m0 + c, live - c, n, s_xs[b] + c, g.ws, g.bias);
         }
-        if (n0 + c >= a.e.n || m0 >= a.e.m) continue;
-        emit_chunk<T, FP8>(a, v, m0, n0 + c, xs, s_ws[b] + c, s_bias[b] + c, s_stage[q]);
+        __syncwarp();
       }
+      if (turn * kChunk >= live) freed();
     }
     __syncwarp();
   }
   if (a.split > 1) {
     cluster_arrive();  // every partial is written
     cluster_wait();
-    // all eight warps where y takes vectors, else the four with a staging buffer
-    if (a.vec || warp >= 4) {
-      const int q = warp & 3, turn = a.vec ? warp >> 2 : 0, turns = a.vec ? 2 : 1;
-      int64_t mi, ni;
-      pair_tile(a, first, &mi, &ni);
-      const int64_t n0 = ni * a.cols, m0 = mi * kPairRows + side * 128 + q * 32, m = m0 + lane;
-      const float xs = FP8 && m < a.e.m ? a.e.xs[m] : 1.f;
-      const float* part = reinterpret_cast<float*>(ring) + q * 32 + lane;
-      for (int c = (pair * turns + turn) * kChunk; c < a.cols && m0 < a.e.m && n0 + c < a.e.n;
-           c += a.split * turns * kChunk) {
-        float v[kChunk] = {};
-        for (int o = 0; o < a.split; ++o) {
-          const uint32_t from = cluster_map(part + c * 128, 2 * o + side);
-          float w[kChunk];  // all on their way before the first is added
-#pragma unroll
-          for (int j = 0; j < kChunk; ++j) w[j] = ld_cluster_f32(from + j * 512);
-#pragma unroll
-          for (int j = 0; j < kChunk; ++j) v[j] += w[j];
-        }
-        emit_chunk<T, FP8>(a, v, m0, n0 + c, xs, s_ws[0] + c, s_bias[0] + c, s_stage[q]);
-      }
-      __syncwarp();
-    }
+    int64_t mi, ni;
+    pair_tile(a, first, &mi, &ni);
+    const int64_t m0 = mi * a.cols;
+    const int live = static_cast<int>(min(static_cast<int64_t>(a.cols), a.e.m - m0));
+    join_parts<T, FP8>(a.e, a.vec, reinterpret_cast<float*>(ring), 128, live, pair, a.split, 2, side, m0,
+                       ni * kPairRows + side * 128, threadIdx.x, kPairThreads);
+    __syncwarp();
   }
   tc_fence_before();
   __syncthreads();
-  cluster_arrive();  // the cluster's last signals, MMAs and reads of partials are over on all sides
+  cluster_arrive_relaxed();  // the cluster's last signals, MMAs and reads of partials are over on all sides
   cluster_wait();
   if (warp == 2) {
     tc_fence_after();
@@ -956,7 +966,7 @@ constexpr size_t kSmemPerTmemCol = 228 * 1024 / 512;
 
 // Clusters of `size` CTAs that fit on the device at once, one CTA per SM.
 template <typename Kern>
-int64_t cluster_slots(Kern kern, int size) {
+int64_t cluster_slots(Kern kern, int threads, int size) {
   static std::mutex mu;
   static std::map<std::tuple<const void*, int, int>, int> known;
   int dev = 0;
@@ -969,7 +979,7 @@ int64_t cluster_slots(Kern kern, int size) {
   int n = 0;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(size));
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1022,9 +1032,10 @@ bool epilogue_vec(const Epilogue& e, int out_dtype, int width) {
 
 // Rows of x up to which the split kernel serves a product.  Each of its CTAs
 // takes in (R + rows of x) * 128 bytes a step, so the pair kernel, which shares
-// the x tile between two CTAs, wins once x is no longer small beside R.  In 16
-// bits, split and pair at 64 / 96 / 128 rows: 4096 x 4096 12.1, 14.5 / 14.2,
-// 14.8 / 15.2, 15.2 us; 28672 x 4096 46.9, 53.3 / 60.3, 54.3 / 62.5, 55.1 us.
+// the x tile between two CTAs, wins once x is no longer small beside R.  Split
+// against pair at 64, 80, 96 and 128 rows: 4096 x 4096 in 16 bits 11.8 / 12.8,
+// 12.6 / 13.5, 14.0 / 13.7, 15.1 / 13.8 us; 28672 x 4096 in 8 bits 24.1 / 24.5,
+// 25.4 / 26.0, 26.6 / 25.1, 29.1 / 26.1 us.
 constexpr int64_t kSplitMaxM = 80;
 
 // Few rows.  FD_ERR_UNSUPPORTED: a layout TMA cannot address.
@@ -1045,7 +1056,7 @@ int launch_split(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t
   while (a.split < kMaxSplit && e.n * a.split * 2 <= static_cast<int64_t>(sms) * kBlockRows && steps >= a.split * 8)
     a.split *= 2;
   // R: equal tiles in one wave of CTAs, or in the fewest
-  const int64_t slots = a.split > 1 ? cluster_slots(product_split_kernel<T, FP8>, a.split) : sms;
+  const int64_t slots = a.split > 1 ? cluster_slots(product_split_kernel<T, FP8>, kSplitThreads, a.split) : sms;
   const int64_t waves = a.split > 1 ? 1 : (e.n + slots * max_rows - 1) / (slots * max_rows);
   const int64_t rows = std::min<int64_t>(((e.n + slots * waves - 1) / (slots * waves) + 7) / 8 * 8, max_rows);
   a.rows = static_cast<int32_t>(rows);
@@ -1090,8 +1101,8 @@ int launch_pair(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t 
   a.box_elems = kBoxBytes / es;
   const int64_t steps = (g.k + a.box_elems - 1) / a.box_elems;
   const int pairs = fd_host::sm_count() / 2;
-  a.mt = (e.m + kPairRows - 1) / kPairRows;
-  // Columns per tile and pairs per tile, by the time they should take: a step
+  a.nt = (e.n + kPairRows - 1) / kPairRows;
+  // Rows of x per tile and pairs per tile, by the time they should take: a step
   // measured 0.12 us + 0.98 ns per column (0.245 at 128 columns, 0.37 at 256,
   // MMAs, L2 and the power limit together), a tile's start and end 0.5 us, the
   // exchange of partials 0.5 us + 6 ns per column.
@@ -1099,43 +1110,48 @@ int launch_pair(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t 
   a.cols = 0;
   a.split = 1;
   for (int split = 1; split <= 4 && (split == 1 || steps >= 4 * split); split *= 2) {
-    const int64_t slots = split > 1 ? cluster_slots(product_pair_kernel<T, FP8>, 2 * split) : pairs;
-    for (int c = kPairCols; c >= 64; c -= kChunk) {
-      const int64_t tiles = a.mt * ((e.n + c - 1) / c);
+    const int64_t slots = split > 1 ? cluster_slots(product_pair_kernel<T, FP8>, kPairThreads, 2 * split) : pairs;
+    for (int64_t most = kPairCols; most >= 32; most -= 32) {
+      const int64_t mt = (e.m + most - 1) / most;
+      const int64_t c = ((e.m + mt - 1) / mt + 31) / 32 * 32;  // as many tiles, evenly filled
+      const int64_t tiles = (e.m + c - 1) / c * a.nt;
       const int64_t waves = (tiles + slots - 1) / slots;
       if (split > 1 && waves > 1) continue;
       const double cost = waves * ((steps + split - 1) / split * (0.12 + 0.00098 * c) + 0.5) +
                           (split > 1 ? 0.5 + 0.006 * c : 0.0);
       if (a.cols == 0 || cost < best) {
         best = cost;
-        a.cols = c;
+        a.cols = static_cast<int32_t>(c);
         a.split = split;
       }
     }
   }
+  a.mt = (e.m + a.cols - 1) / a.cols;
   a.group = 16;
-  a.nt = (e.n + a.cols - 1) / a.cols;
-  if (steps > 0x7fffffffLL || e.m > 0x7fffff00LL || e.n > 0x7fffff00LL) return FD_ERR_UNSUPPORTED;
+  if (steps > 0x7fffffffLL || e.m > 0x7fffff00LL || e.n > 0x7fffff00LL || (a.mt + 16) * a.nt > 0x7fffffffLL)
+    return FD_ERR_UNSUPPORTED;
   a.steps = static_cast<int32_t>(steps);
   a.desc = mma_desc(FP8 ? 0 : mma_format(in_dtype), kPairRows, a.cols);
-  a.vec = e.n % 8 == 0 && epilogue_vec(e, out_dtype, 8);
+  a.vec = epilogue_vec(e, out_dtype, 4);
   const size_t stage = static_cast<size_t>(kBoxBytes) * (128 + a.cols / 2);
-  a.stages = static_cast<int32_t>(std::min<size_t>(kMaxRing, 192 * 1024 / stage));
+  a.stages = static_cast<int32_t>(std::min<size_t>(kMaxRing, 216 * 1024 / stage));
   // all of an SM's shared memory, as all of its tensor memory
-  const size_t smem = std::max<size_t>(a.stages * stage + 1024, 204 * 1024);
-  CUtensorMap xm, wm;
-  if (!operand_map(&xm, g.x, e.m, g.k, g.sxm, g.sxk, es, 128) ||
-      !operand_map(&wm, g.w, e.n, g.k, g.swn, g.swk, es, a.cols / 2))
+  const size_t smem = std::max<size_t>(a.stages * stage + 1024, 217 * 1024);
+  CUtensorMap wm, xm;
+  if (!operand_map(&wm, g.w, e.n, g.k, g.swn, g.swk, es, 128) ||
+      !operand_map(&xm, g.x, e.m, g.k, g.sxm, g.sxk, es, a.cols / 2))
     return FD_ERR_UNSUPPORTED;
   const int64_t grid = 2 * a.split * (a.split > 1 ? a.mt * a.nt : std::min<int64_t>(pairs, a.mt * a.nt));
   return from_cuda(launch_cluster(product_pair_kernel<T, FP8>, dim3(static_cast<unsigned>(grid)), kPairThreads,
-                                  2 * a.split, smem, st, xm, wm, a));
+                                  2 * a.split, smem, st, wm, xm, a));
 }
 
 template <typename TX, typename T, bool FP8>
 int launch_product(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t st) {
   int r = FD_ERR_UNSUPPORTED;
-  if (g.k > 0) {
+  // emit_some's 32-bit column offsets
+  const bool near = g.epi.sym >= 0 && g.epi.srm >= 0 && std::max(g.epi.sym, g.epi.srm) < (int64_t{1} << 27);
+  if (g.k > 0 && near) {
     r = g.epi.m <= kSplitMaxM ? launch_split<T, FP8>(g, in_dtype, out_dtype, st)
                               : launch_pair<T, FP8>(g, in_dtype, out_dtype, st);
   }
