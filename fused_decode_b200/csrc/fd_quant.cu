@@ -41,6 +41,24 @@ struct QuantArgs {
   float eps;
 };
 
+// silu(g) * u by the hardware's exp2 and reciprocal, flushing subnormals: for
+// g towards -inf the exponential overflows to infinity and the sigmoid to 0.
+// The exponential's error grows with its argument: relative 2^-22 and
+// |g| 2^-24, where the row is rounded to 2^-4.
+FD_DEV float silu_mul_fast(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
+}
+
+// max(a, |b|) that keeps a NaN.
+FD_DEV float max_abs(float a, float b) {
+  float v;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(a), "f"(fabsf(b)));
+  return v;
+}
+
 FD_DEV uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // The floor under the row maximum (a NaN stays one).
@@ -87,7 +105,7 @@ __global__ void __launch_bounds__(kGenThreads) quant_generic_kernel(QuantArgs a)
   auto raw = [&](int64_t j) {
     const float v = to_f32(xr[j * a.x.col]);
     if (OP == ROW_ADD_RMS) return v + to_f32(rr[j * a.r.col]);
-    if (OP == ROW_SWIGLU) return silu_mul(v, to_f32(rr[j * a.r.col]));
+    if (OP == ROW_SWIGLU) return silu_mul_fast(v, to_f32(rr[j * a.r.col]));
     return v;
   };
   float inv = 1.f;
@@ -133,13 +151,13 @@ struct QuantVecArgs {
 
 struct RowStats {
   float sum;
-  uint32_t top;
+  float top;  // maximum of the magnitudes
 };
 
 // Sum and maximum over the warps of a row's group; every warp of the CTA takes part.
-FD_DEV RowStats group_reduce(RowStats s, int wpr, int group, float* red_sum, uint32_t* red_top) {
+FD_DEV RowStats group_reduce(RowStats s, int wpr, int group, float* red_sum, float* red_top) {
   s.sum = warp_sum(s.sum);
-  s.top = __reduce_max_sync(0xffffffffu, s.top);
+  s.top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s.top)));
   if (wpr > 1) {
     const int warp = threadIdx.x >> 5;
     if ((threadIdx.x & 31) == 0) {
@@ -147,10 +165,10 @@ FD_DEV RowStats group_reduce(RowStats s, int wpr, int group, float* red_sum, uin
       red_top[warp] = s.top;
     }
     __syncthreads();
-    s = {0.f, 0u};
+    s = {0.f, 0.f};
     for (int w = 0; w < wpr; ++w) {
       s.sum += red_sum[group * wpr + w];
-      s.top = max(s.top, red_top[group * wpr + w]);
+      s.top = max_abs(s.top, red_top[group * wpr + w]);
     }
   }
   return s;
@@ -163,118 +181,139 @@ FD_DEV uint2 pack8_e4m3(const float* f) {
   return make_uint2(two(f[0], f[1]) | two(f[2], f[3]) << 16, two(f[4], f[5]) | two(f[6], f[7]) << 16);
 }
 
+// A row in registers, VPT vectors to a thread (vector j = t + i * threads): its
+// statistics, then its values.
+template <typename T, int OP, int VPT>
+struct RowRegs {
+  static constexpr bool kNorm = OP == ROW_RMS || OP == ROW_ADD_RMS;
+  static constexpr bool kTwo = OP == ROW_ADD_RMS || OP == ROW_SWIGLU;
+  float s[VPT][8];  // the row before the norm's scale and weight
+  uint4 w16[VPT];   // the norm weight, where it is of 16 bits
+
+  // issued with the row's loads, not after they have arrived
+  FD_DEV void ask_weight(const QuantArgs& g, int i, int j) {
+    if (kNorm && g.w_dtype != FD_F32) w16[i] = __ldg(static_cast<const uint4*>(g.w) + j);
+  }
+  FD_DEV void weight(const QuantArgs& g, int i, int j, float* w) const {
+    if (g.w_dtype == FD_F32) load8_as_f32(static_cast<const float*>(g.w) + 8 * j, FD_F32, w);
+    else if (g.w_dtype == FD_BF16) unpack8<__nv_bfloat16>(w16[i], w);
+    else unpack8<__half>(w16[i], w);
+  }
+  // vector i (the row's vector j) from its packed inputs
+  FD_DEV void take(const QuantArgs& g, int i, int j, const uint4& x, const uint4& r, RowStats* st) {
+    unpack8<T>(x, s[i]);
+    if (kTwo) {
+      float f[8];
+      unpack8<T>(r, f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[i][e] = OP == ROW_SWIGLU ? silu_mul_fast(s[i][e], f[e]) : s[i][e] + f[e];
+    }
+    if (kNorm) {
+      float w[8];
+      weight(g, i, j, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        st->sum += s[i][e] * s[i][e];
+        st->top = max_abs(st->top, s[i][e] * w[e]);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) st->top = max_abs(st->top, s[i][e]);
+    }
+  }
+  // (row maximum, 1 / rms) from the row's statistics.  Where s * w overflowed,
+  // or holds an infinity or a NaN, `again` reduces the maximum of the products
+  // themselves, as the definition orders them.
+  template <typename Again>
+  FD_DEV float amax(const QuantArgs& g, RowStats st, int t, int threads, int nv, bool live, float* inv, Again again) {
+    if (!kNorm) return st.top;
+    *inv = rsqrtf(st.sum / static_cast<float>(g.n) + g.eps);
+    if (st.top < __uint_as_float(0x7f800000u)) return st.top * *inv;
+    RowStats more{0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = t + i * threads;
+      if (live && j < nv) {
+        float w[8];
+        weight(g, i, j, w);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) more.top = max_abs(more.top, s[i][e] * *inv * w[e]);
+      }
+    }
+    return again(more).top;
+  }
+  FD_DEV void put(const QuantArgs& g, int i, int j, float inv, float up, uint8_t* q) const {
+    float o[8];
+    if (kNorm) {
+      float w[8];
+      weight(g, i, j, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = s[i][e] * inv * w[e] * up;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = s[i][e] * up;
+    }
+    *reinterpret_cast<uint2*>(q + 8 * j) = pack8_e4m3(o);
+  }
+};
+
 template <typename T, int OP, int VPT, bool FLAT>
-__global__ void __launch_bounds__(512) quant_vec_kernel(QuantVecArgs a) {
-  __shared__ float red_sum[2][16];
-  __shared__ uint32_t red_top[2][16];
-  constexpr bool kNorm = OP == ROW_RMS || OP == ROW_ADD_RMS;
-  constexpr bool kTwo = OP == ROW_ADD_RMS || OP == ROW_SWIGLU;
+__global__ void __launch_bounds__(1024) quant_vec_kernel(QuantVecArgs a) {
+  __shared__ float red_sum[2][32], red_top[2][32];
+  using Row = RowRegs<T, OP, VPT>;
   const int group_threads = 32 * a.wpr;
   const int group = threadIdx.x / group_threads;
   const int t = threadIdx.x - group * group_threads;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * a.rpc + group;
   const bool live = row < a.g.rows;
   const RowIdx ri = split_row<FLAT>(live ? row : 0, a.g.B, a.g.C);
-  const int wes = a.g.w_dtype == FD_F32 ? 4 : 2;
-  auto weight = [&](int j, float* w) {
-    load8_as_f32(static_cast<const char*>(a.g.w) + static_cast<int64_t>(8 * j) * wes, a.g.w_dtype, w);
-  };
   grid_dep_wait();
   grid_dep_launch();
 
-  float s[VPT][8];
-  RowStats st{0.f, 0u};
+  Row v;
+  RowStats st{0.f, 0.f};
   if (live) {
     const T* xr = reinterpret_cast<const T*>(a.g.x.ptr) + offset_of(a.g.x, ri);
-    const T* rr = kTwo ? reinterpret_cast<const T*>(a.g.r.ptr) + offset_of(a.g.r, ri) : nullptr;
+    const T* rr = Row::kTwo ? reinterpret_cast<const T*>(a.g.r.ptr) + offset_of(a.g.r, ri) : nullptr;
     uint4 xv[VPT], rv[VPT];
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int j = t + i * group_threads;
       if (j < a.nv) {
         xv[i] = ld_plain16(xr + 8 * j);
-        if (kTwo) rv[i] = ld_plain16(rr + 8 * j);
+        if (Row::kTwo) rv[i] = ld_plain16(rr + 8 * j);
+        v.ask_weight(a.g, i, j);
       }
     }
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int j = t + i * group_threads;
-      if (j < a.nv) {
-        unpack8<T>(xv[i], s[i]);
-        if (kTwo) {
-          float f[8];
-          unpack8<T>(rv[i], f);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) s[i][e] = OP == ROW_SWIGLU ? silu_mul(s[i][e], f[e]) : s[i][e] + f[e];
-        }
-        if (kNorm) {
-          float w[8];
-          weight(j, w);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            st.sum += s[i][e] * s[i][e];
-            st.top = max(st.top, abs_bits(s[i][e] * w[e]));
-          }
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) st.top = max(st.top, abs_bits(s[i][e]));
-        }
-      }
+      if (j < a.nv) v.take(a.g, i, j, xv[i], rv[i], &st);
     }
     if (OP == ROW_ADD_RMS) {
       T* ror = reinterpret_cast<T*>(a.g.ro.ptr) + offset_of(a.g.ro, ri);
 #pragma unroll
       for (int i = 0; i < VPT; ++i) {
         const int j = t + i * group_threads;
-        if (j < a.nv) st_stream16(ror + 8 * j, pack8<T>(s[i]));
+        if (j < a.nv) st_stream16(ror + 8 * j, pack8<T>(v.s[i]));
       }
     }
   }
   st = group_reduce(st, a.wpr, group, red_sum[0], red_top[0]);
-  float inv = 1.f, amax = __uint_as_float(st.top);
-  if (kNorm) {
-    inv = rsqrtf(st.sum / static_cast<float>(a.g.n) + a.g.eps);
-    if (st.top < 0x7f800000u) {
-      amax *= inv;
-    } else {
-      // s * w overflowed, or holds an infinity or a NaN: the maximum of the
-      // products themselves, as the definition orders them.  With one warp a
-      // row the condition may differ between a CTA's rows, and the reduction
-      // stays within the warp; with more there is one row to a CTA.
-      RowStats again{0.f, 0u};
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int j = t + i * group_threads;
-        if (live && j < a.nv) {
-          float w[8];
-          weight(j, w);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) again.top = max(again.top, abs_bits(s[i][e] * inv * w[e]));
-        }
-      }
-      amax = __uint_as_float(group_reduce(again, a.wpr, group, red_sum[1], red_top[1]).top);
-    }
-  }
+  // With one warp a row, whether the maximum is reduced again may differ
+  // between a CTA's rows, and stays within the warp; with more there is one row
+  // to a CTA.
+  float inv = 1.f;
+  const float amax = floor_amax(v.amax(a.g, st, t, group_threads, a.nv, live, &inv, [&](RowStats more) {
+    return group_reduce(more, a.wpr, group, red_sum[1], red_top[1]);
+  }));
   if (!live) return;
-  amax = floor_amax(amax);
   const float up = kMax8 / amax;
   uint8_t* qr = reinterpret_cast<uint8_t*>(a.g.q.ptr) + offset_of(a.g.q, ri);
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int j = t + i * group_threads;
-    if (j < a.nv) {
-      float o[8];
-      if (kNorm) {
-        float w[8];
-        weight(j, w);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = s[i][e] * inv * w[e] * up;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = s[i][e] * up;
-      }
-      *reinterpret_cast<uint2*>(qr + 8 * j) = pack8_e4m3(o);
-    }
+    if (j < a.nv) v.put(a.g, i, j, inv, up, qr);
   }
   if (t == 0) a.g.scale[row] = amax / kMax8;
 }
@@ -296,7 +335,10 @@ cudaError_t launch_vec2(const QuantVecArgs& a, bool flat, cudaStream_t st) {
               : fd_host::launch_pdl(quant_vec_kernel<T, OP, VPT, false>, blocks, threads, 0, st, a);
 }
 
-// Vectors per thread and warps per row, nv <= 4096.
+// Vectors per thread and warps per row, nv <= 4096.  Many rows run best with four
+// vectors to a thread (add_rms_norm_fp8 8192 x 4096: 42.2 us, with one, two or
+// eight 59, 45, 49), few rows with as many threads a row as a CTA may have (1 x
+// 4096: 2.3 us, with four vectors 3.3).
 template <typename T, int OP>
 cudaError_t launch_vec(QuantVecArgs a, bool flat, cudaStream_t st) {
   const int nv = a.nv;
@@ -306,21 +348,17 @@ cudaError_t launch_vec(QuantVecArgs a, bool flat, cudaStream_t st) {
   if (nv <= 64) return launch_vec2<T, OP, 2>(a, flat, st);
   a.rpc = 1;
   auto warps = [&](int vpt) { return (nv + 32 * vpt - 1) / (32 * vpt); };
-  // few rows: as many threads a row as a CTA has, for the shortest chain
-  if (a.g.rows <= fd_host::sm_count() && warps(1) <= 16) {
+  const bool few = a.g.rows <= fd_host::sm_count();
+  if (few && warps(1) <= 16) {
     a.wpr = warps(1);
     return launch_vec2<T, OP, 1>(a, flat, st);
   }
-  if (a.g.rows <= fd_host::sm_count() && warps(2) <= 16) {
+  if (few && warps(2) <= 16) {
     a.wpr = warps(2);
     return launch_vec2<T, OP, 2>(a, flat, st);
   }
-  if (warps(4) <= 16) {
-    a.wpr = warps(4);
-    return launch_vec2<T, OP, 4>(a, flat, st);
-  }
-  a.wpr = warps(8);
-  return launch_vec2<T, OP, 8>(a, flat, st);
+  a.wpr = warps(4);  // <= 32
+  return launch_vec2<T, OP, 4>(a, flat, st);
 }
 
 template <int OP>
