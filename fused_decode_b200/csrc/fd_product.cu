@@ -236,7 +236,7 @@ FD_DEV void tc_commit(uint64_t* bar, uint16_t mask = 0) {
         : "memory");
 }
 
-// 16 / 32 consecutive accumulator columns of this warp's 32 lanes (tcgen05.ld
+// 16 consecutive accumulator columns of this warp's 32 lanes (tcgen05.ld
 // reads lanes 32 * (warp % 4) + lane), arrived on return: the wait is in the
 // same statement, so that no use of the values can be moved before it.
 FD_DEV void tc_load16(uint32_t addr, uint32_t* v) {
@@ -247,15 +247,6 @@ FD_DEV void tc_load16(uint32_t addr, uint32_t* v) {
       : "r"(addr)
       : "memory");
 }
-FD_DEV void tc_load32(uint32_t addr, uint32_t* v) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(addr)
-      : "memory");
-}
-
 // One lane of a converged warp, chosen by elect.sync.  TMA and tcgen05
 // instructions take warp-uniform operands; issued under `if (lane == 0)`
 // instead, a step of four MMAs and its commit measured about 700 cycles whatever
@@ -685,8 +676,11 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
 // through distributed shared memory.
 constexpr int kPairRows = 256;
 constexpr int kPairCols = 256;     // at most
-constexpr int kPairThreads = 384;  // TMA, MMA, tensor memory, idle; eight epilogue warps
-constexpr int kChunk = 32;         // accumulator columns an epilogue warp handles at once
+constexpr int kEpilogueWarps = 8;  // a multiple of 4: warp w reads the tensor memory lanes of w % 4
+constexpr int kPairThreads = 128 + 32 * kEpilogueWarps;  // TMA, MMA, tensor memory, one idle warp
+// Accumulator columns an epilogue warp handles at once: with 32 the code of a
+// chunk is as long again and 8192 x 4096 x 512 takes 34 us, with 16 it takes 30.
+constexpr int kChunk = 16;
 
 struct PairArgs {
   Epilogue e;
@@ -753,7 +747,7 @@ __global__ void __launch_bounds__(kPairThreads, 1)
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);
-      mbar_init(&acc_empty[b], 16);  // eight epilogue warps of each CTA
+      mbar_init(&acc_empty[b], 2 * kEpilogueWarps);  // of both CTAs
     }
     abort = 0;
     bar_init_fence();
@@ -859,10 +853,21 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         if (FP8) g.ws = a.e.ws[g.n];
         if (a.e.bias) g.bias = load_as_f32(a.e.bias, a.e.bias_dtype, g.n * a.e.sbias);
       }
-      if (FP8 && et < g.live) g.xs = a.e.xs[g.m0 + et];
+      if (et < g.live) {
+        if (FP8) g.xs = a.e.xs[g.m0 + et];
+        // row et of the tile's part of row_add into L2: the loads themselves keep
+        // too few bytes in flight for HBM's latency
+        if (a.e.ra && a.e.srn == 1 && a.e.srm != 0) {
+          const int es = a.e.ra_dtype == FD_F32 ? 4 : 2;
+          const int64_t n0 = ni * kPairRows + side * 128;
+          const char* p = static_cast<const char*>(a.e.ra) + ((g.m0 + et) * a.e.srm + n0) * es;
+          const int bytes = static_cast<int>(min(int64_t{128}, a.e.n - n0)) * es;
+          for (int o = 0; o < bytes; o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + o));
+        }
+      }
       return g;
     };
-    static_assert(kPairCols == kPairThreads - 128, "one row of x to a thread");
+    static_assert(kPairCols <= 32 * kEpilogueWarps, "one row of x to a thread");
     int it = 0;
     bool ok = true;
     Edge next = edge_of(first);
@@ -873,11 +878,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
       const int live = g.live;
       const bool row_ok = n < a.e.n;
       if (FP8) {
-        s_xs[b][et] = g.xs;
-        named_sync(1, 256);
+        if (et < kPairCols) s_xs[b][et] = g.xs;
+        named_sync(1, 32 * kEpilogueWarps);
       }
       next = edge_of(t + stride);
-      // after an expired wait the eight warps still meet at every tile's barrier
+      // after an expired wait the warps still meet at every tile's barrier
       ok = ok && wait_or_abort(&acc_full[b], (it >> 1) & 1, &abort);
       if (!ok) continue;
       tc_fence_after();
@@ -889,10 +894,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         if (lane == 0) arrive_cluster(cluster_map(&acc_empty[b], crank - side));
       };
-      for (int c = turn * kChunk; c < live; c += 2 * kChunk) {
+      constexpr int kRound = kEpilogueWarps / 4 * kChunk;
+      for (int c = turn * kChunk; c < live; c += kRound) {
         float v[kChunk];
-        tc_load32(acc + c, reinterpret_cast<uint32_t*>(v));
-        if (c + 2 * kChunk >= live) freed();
+        tc_load16(acc + c, reinterpret_cast<uint32_t*>(v));
+        if (c + kRound >= live) freed();
         if (a.split > 1) {
 #pragma unroll
           for (int j = 0; j < kChunk; ++j)
