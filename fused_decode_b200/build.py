@@ -80,7 +80,7 @@ def build_fastpath(force: bool = False, verbose: bool = False) -> str:
     tmp = FASTPATH_OUT + ".tmp"
     cmd += [FASTPATH_SRC, "-o", tmp, "-L", HERE, "-lfd_b200", "-Wl,-rpath,$ORIGIN",
             "-L", torch_lib, f"-Wl,-rpath,{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu",
-            "-ltorch_python"]
+            "-ltorch_cuda", "-ltorch_python"]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -17,6 +17,7 @@
 // The split-K workspaces (one zero-filled buffer per device and stream) live
 // here and serve both paths.
 #include <ATen/core/Tensor.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/linear.h>
 #include <ATen/ops/zeros.h>
@@ -423,11 +424,16 @@ py::object post_attn_mlp(py::handle hh, py::handle hnw, py::handle hgu, py::hand
 }
 
 // ------------------------------------------------------------ 8-bit rows
+// A fresh contiguous tensor beside `like`, without the dispatcher's part of at::empty.
+at::Tensor fresh(c10::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+
 // ops_fp8.py's outputs: given ones must be what the kernels can write in
 // place, absent ones are fresh.
 bool rows8_for(py::handle hout, py::handle hscale, const at::Tensor& x, at::Tensor* q, at::Tensor* scale, fd_rows* rq) {
   if (hout.is_none()) {
-    *q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+    *q = fresh(x.sizes(), at::kFloat8_e4m3fn, x);
   } else {
     const at::Tensor* o = as_tensor(hout);
     if (!o || o->sizes() != x.sizes() || o->scalar_type() != at::kFloat8_e4m3fn || o->device() != x.device())
@@ -438,7 +444,7 @@ bool rows8_for(py::handle hout, py::handle hscale, const at::Tensor& x, at::Tens
   rq->dtype = FD_E4M3;
   const c10::IntArrayRef lead = x.sizes().slice(0, x.dim() - 1);
   if (hscale.is_none()) {
-    *scale = at::empty(lead, x.options().dtype(at::kFloat));
+    *scale = fresh(lead, at::kFloat, x);
   } else {
     const at::Tensor* o = as_tensor(hscale);
     if (!o || o->sizes() != lead || o->scalar_type() != at::kFloat || o->device() != x.device() || !o->is_contiguous())
@@ -489,7 +495,13 @@ py::object add_rms_norm_fp8(py::handle hx, py::handle hr, py::handle hw, py::han
     return py::none();
   const c10::cuda::CUDAGuard guard(x->device());
   at::Tensor q, scale, res_out;
-  if (!rows8_for(hout, hscale, *x, &q, &scale, &rq) || !out_for(hres_out, *x, &res_out, &rro)) return py::none();
+  if (!rows8_for(hout, hscale, *x, &q, &scale, &rq)) return py::none();
+  if (hres_out.is_none()) {
+    res_out = fresh(x->sizes(), x->scalar_type(), *x);
+    if (!rows_of(res_out, &rro)) return py::none();
+  } else if (!out_for(hres_out, *x, &res_out, &rro)) {
+    return py::none();
+  }
   if (row_count(rx) > 0)
     check(fd_rms_fp8_out(&rx, &rr, w->data_ptr(), dtype_code(w->scalar_type()), w->stride(0), &rq,
                          scale.data_ptr<float>(), &rro, static_cast<float>(eps), stream_of(*x)),
@@ -566,7 +578,7 @@ bool product_call(const at::Tensor& x, const at::Tensor& w, py::handle hb, py::h
     c->ra_dt = dtype_code(ra->scalar_type());
   }
   if (hout.is_none()) {
-    c->y = at::empty(expected, x.options().dtype(out_type));
+    c->y = fresh(expected, out_type, x);
     return true;
   }
   const at::Tensor* o = as_tensor(hout);
@@ -637,9 +649,9 @@ py::object post_attn_mlp_fp8(py::handle hh, py::handle hnw, py::handle hgu, py::
   int64_t m, s_hidden, sxk;
   if (!as_mk(*hid, &m, &s_hidden, &sxk) || m < 1 || sxk != 1) return py::none();
   const c10::cuda::CUDAGuard guard(hid->device());
-  at::Tensor out = at::empty(hid->sizes(), hid->options());
+  at::Tensor out = fresh(hid->sizes(), hid->scalar_type(), *hid);
   const size_t bytes = fd_post_attn_mlp_fp8_workspace_bytes(m, h, i);
-  const at::Tensor ws = at::empty({static_cast<int64_t>(bytes)}, hid->options().dtype(at::kByte));
+  const at::Tensor ws = fresh({static_cast<int64_t>(bytes)}, at::kByte, *hid);
   check(fd_post_attn_mlp_fp8_out(hid->data_ptr(), s_hidden, nw->data_ptr(), dtype_code(nw->scalar_type()),
                                  nw->stride(0), wgu->data_ptr(), wgu->stride(0), gs->data_ptr<float>(), wd->data_ptr(),
                                  wd->stride(0), ds->data_ptr<float>(), out.data_ptr(), dtype_code(hid->scalar_type()), m,

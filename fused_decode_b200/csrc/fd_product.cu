@@ -7,9 +7,7 @@
 #include <cuda_fp8.h>
 
 #include <algorithm>
-#include <map>
-#include <mutex>
-#include <tuple>
+#include <atomic>
 #include <type_traits>
 
 using namespace fd;
@@ -266,6 +264,9 @@ FD_DEV void tma_prefetch_2d(const CUtensorMap* map, int32_t x, int32_t y) {
                "r"(x), "r"(y)
                : "memory");
 }
+
+FD_DEV void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+FD_DEV int dtype_size(int dtype) { return dtype == FD_F32 ? 4 : 2; }
 
 FD_DEV void bar_init_fence() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 FD_DEV void named_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -585,6 +586,24 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
   grid_dep_wait();
   grid_dep_launch();
   const int live = static_cast<int>(a.e.m);  // columns in use
+  if (warp >= 4) {  // the first tile's part of the epilogue's operands into L2, under its MMAs
+    const int et = threadIdx.x - 128;
+    const int64_t n0 = first * a.rows;
+    const int rows = static_cast<int>(min(static_cast<int64_t>(a.rows), a.e.n - n0));
+    for (int r = et; r < rows; r += 128) {
+      if (FP8) prefetch_l2(a.e.ws + n0 + r);
+      if (a.e.bias) prefetch_l2(static_cast<const char*>(a.e.bias) + (n0 + r) * a.e.sbias * dtype_size(a.e.bias_dtype));
+    }
+    if (et < live) {
+      if (FP8) prefetch_l2(a.e.xs + et);
+      if (a.e.ra && a.e.srn == 1 && et % a.split == static_cast<int>(rank)) {
+        const int es = dtype_size(a.e.ra_dtype);
+        const char* p = static_cast<const char*>(a.e.ra) + (et * a.e.srm + n0) * es;
+        for (int o = 0; o < rows * es; o += 128) prefetch_l2(p + o);
+      }
+    }
+    __syncwarp();
+  }
   if (a.split == 1) {
     // straight from tensor memory: a thread per row of the tile
     if (warp >= 4) {
@@ -592,6 +611,15 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
       int it = 0;
       for (int64_t t = first; t < a.tiles; t += stride, ++it) {
         const int b = a.accs == 2 ? it & 1 : 0, turn = a.accs == 2 ? it >> 1 : it;
+        float ws2[2] = {1.f, 1.f}, bias2[2] = {0.f, 0.f};  // of this thread's row in either block
+#pragma unroll
+        for (int blk = 0; blk < 2; ++blk) {
+          const int r = blk * kBlockRows + (warp - 4) * 32 + lane;
+          const int64_t n = t * a.rows + r;
+          if (r >= a.rows || n >= a.e.n) continue;
+          if (FP8) ws2[blk] = a.e.ws[n];
+          if (a.e.bias) bias2[blk] = load_as_f32(a.e.bias, a.e.bias_dtype, n * a.e.sbias);
+        }
         ok = ok && wait_or_abort(&acc_full[b], turn & 1, &abort);
         if (!ok) break;
         tc_fence_after();
@@ -599,8 +627,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
           const int r = blk * kBlockRows + (warp - 4) * 32 + lane;
           const int64_t n = t * a.rows + r;
           const bool row_ok = r < a.rows && n < a.e.n;
-          const float ws = FP8 && row_ok ? a.e.ws[n] : 1.f;
-          const float bias = a.e.bias && row_ok ? load_as_f32(a.e.bias, a.e.bias_dtype, n * a.e.sbias) : 0.f;
+          const float ws = blk ? ws2[1] : ws2[0], bias = blk ? bias2[1] : bias2[0];
           const uint32_t acc = tmem + (static_cast<uint32_t>((warp - 4) * 32) << 16) + b * acc_cols + blk * a.cols;
           for (int c = 0; c < live; c += 16) {
             float v[16], xs[16];
@@ -858,11 +885,11 @@ __global__ void __launch_bounds__(kPairThreads, 1)
         // row et of the tile's part of row_add into L2: the loads themselves keep
         // too few bytes in flight for HBM's latency
         if (a.e.ra && a.e.srn == 1 && a.e.srm != 0) {
-          const int es = a.e.ra_dtype == FD_F32 ? 4 : 2;
+          const int es = dtype_size(a.e.ra_dtype);
           const int64_t n0 = ni * kPairRows + side * 128;
           const char* p = static_cast<const char*>(a.e.ra) + ((g.m0 + et) * a.e.srm + n0) * es;
           const int bytes = static_cast<int>(min(int64_t{128}, a.e.n - n0)) * es;
-          for (int o = 0; o < bytes; o += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(p + o));
+          for (int o = 0; o < bytes; o += 128) prefetch_l2(p + o);
         }
       }
       return g;
@@ -963,66 +990,79 @@ bool operand_map(CUtensorMap* map, const void* p, int64_t rows, int64_t k, int64
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-constexpr size_t kSmemMax = 227 * 1024;
+constexpr size_t kSplitSmemMax = 226 * 1024;
+constexpr size_t kPairSmem = 217 * 1024;  // all of an SM's, as it takes all of its tensor memory
 // Tensor memory has 512 columns an SM and an allocation waits for them.  A CTA
 // takes at least this much shared memory for each column, its share of the
 // SM's 228 KB: no SM ever holds CTAs that want more columns than there are, so
 // no allocation waits for a CTA that is itself waiting for a peer.
 constexpr size_t kSmemPerTmemCol = 228 * 1024 / 512;
 
-// Clusters of `size` CTAs that fit on the device at once, one CTA per SM.
-template <typename Kern>
-int64_t cluster_slots(Kern kern, int threads, int size) {
-  static std::mutex mu;
-  static std::map<std::tuple<const void*, int, int>, int> known;
+constexpr int kMaxDevices = 64;
+
+// Let a kernel have up to `bytes` of dynamic shared memory: once per device.
+template <auto kKernel>
+cudaError_t allow_smem(size_t bytes) {
+  static std::atomic<bool> done[kMaxDevices];
   int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-  const auto key = std::make_tuple(reinterpret_cast<const void*>(kern), dev, size);
-  std::lock_guard<std::mutex> lock(mu);
-  auto it = known.find(key);
-  if (it != known.end()) return it->second;
-  const size_t smem = 200 * 1024;
-  int n = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < kMaxDevices && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+  e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(bytes));
+  if (e == cudaSuccess && dev < kMaxDevices) done[dev].store(true, std::memory_order_release);
+  return e;
+}
+
+void set_cluster(cudaLaunchAttribute* attr, int size) {
+  attr->id = cudaLaunchAttributeClusterDimension;
+  attr->val.clusterDim.x = static_cast<unsigned>(size);
+  attr->val.clusterDim.y = 1;
+  attr->val.clusterDim.z = 1;
+}
+
+// Clusters of `size` CTAs (2 to 8) that fit on the device at once, one CTA per
+// SM: asked once per device.
+template <auto kKernel>
+int64_t cluster_slots(int threads, size_t smem, int size) {
+  static std::atomic<int> known[kMaxDevices][9];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= kMaxDevices) return 1;
+  int n = known[dev][size].load(std::memory_order_relaxed);
+  if (n > 0) return n;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(size));
   cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = static_cast<unsigned>(size);
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
+  set_cluster(&attr[0], size);
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) != cudaSuccess ||
-      cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
+  if (allow_smem<kKernel>(smem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kKernel, &cfg) != cudaSuccess ||
+      n < 1) {
     (void)cudaGetLastError();
     n = 1;
   }
-  known[key] = n;
+  known[dev][size].store(n, std::memory_order_relaxed);
   return n;
 }
 
-template <typename Kern, typename Args>
-cudaError_t launch_cluster(Kern kern, dim3 grid, int threads, int cluster, size_t smem, cudaStream_t st,
+template <auto kKernel, typename Args>
+cudaError_t launch_cluster(dim3 grid, int threads, int cluster, size_t smem, size_t smem_max, cudaStream_t st,
                            const CUtensorMap& m0, const CUtensorMap& m1, const Args& a) {
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  const cudaError_t e = allow_smem<kKernel>(smem_max);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
-  attr[1].id = cudaLaunchAttributeClusterDimension;
-  attr[1].val.clusterDim.x = static_cast<unsigned>(cluster);
-  attr[1].val.clusterDim.y = 1;
-  attr[1].val.clusterDim.z = 1;
+  set_cluster(&attr[1], cluster);
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kern, m0, m1, a);
+  return cudaLaunchKernelEx(&cfg, kKernel, m0, m1, a);
 }
 
 int mma_format(int in_dtype) { return in_dtype == FD_BF16 ? 1 : 0; }
@@ -1062,7 +1102,7 @@ int launch_split(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t
   while (a.split < kMaxSplit && e.n * a.split * 2 <= static_cast<int64_t>(sms) * kBlockRows && steps >= a.split * 8)
     a.split *= 2;
   // R: equal tiles in one wave of CTAs, or in the fewest
-  const int64_t slots = a.split > 1 ? cluster_slots(product_split_kernel<T, FP8>, kSplitThreads, a.split) : sms;
+  const int64_t slots = a.split > 1 ? cluster_slots<product_split_kernel<T, FP8>>(kSplitThreads, kSplitSmemMax, a.split) : sms;
   const int64_t waves = a.split > 1 ? 1 : (e.n + slots * max_rows - 1) / (slots * max_rows);
   const int64_t rows = std::min<int64_t>(((e.n + slots * waves - 1) / (slots * waves) + 7) / 8 * 8, max_rows);
   a.rows = static_cast<int32_t>(rows);
@@ -1088,14 +1128,14 @@ int launch_split(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t
   // an MMA reads whole blocks of 128 rows, past the last stage's R
   const size_t reads = (a.stages - 1) * stage + static_cast<size_t>(kBoxBytes) * a.blocks * kBlockRows;
   const size_t smem = std::max(a.tmem_cols * kSmemPerTmemCol, std::max(std::max(a.stages * stage, reads), part) + 1024);
-  if (smem > kSmemMax - 1024) return FD_ERR_UNSUPPORTED;
+  if (smem > kSplitSmemMax) return FD_ERR_UNSUPPORTED;
   CUtensorMap wm, xm;
   if (!operand_map(&wm, g.w, e.n, g.k, g.swn, g.swk, es, a.rows) ||
       !operand_map(&xm, g.x, e.m, g.k, g.sxm, g.sxk, es, a.cols))
     return FD_ERR_UNSUPPORTED;
   const int64_t grid = a.split > 1 ? a.tiles * a.split : std::min<int64_t>(a.tiles, sms);
-  return from_cuda(launch_cluster(product_split_kernel<T, FP8>, dim3(static_cast<unsigned>(grid)), kSplitThreads,
-                                  a.split, smem, st, wm, xm, a));
+  return from_cuda(launch_cluster<product_split_kernel<T, FP8>>(dim3(static_cast<unsigned>(grid)), kSplitThreads,
+                                                                a.split, smem, kSplitSmemMax, st, wm, xm, a));
 }
 
 template <typename T, bool FP8>
@@ -1116,7 +1156,7 @@ int launch_pair(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t 
   a.cols = 0;
   a.split = 1;
   for (int split = 1; split <= 4 && (split == 1 || steps >= 4 * split); split *= 2) {
-    const int64_t slots = split > 1 ? cluster_slots(product_pair_kernel<T, FP8>, kPairThreads, 2 * split) : pairs;
+    const int64_t slots = split > 1 ? cluster_slots<product_pair_kernel<T, FP8>>(kPairThreads, kPairSmem, 2 * split) : pairs;
     for (int64_t most = kPairCols; most >= 32; most -= 32) {
       const int64_t mt = (e.m + most - 1) / most;
       const int64_t c = ((e.m + mt - 1) / mt + 31) / 32 * 32;  // as many tiles, evenly filled
@@ -1141,15 +1181,13 @@ int launch_pair(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t 
   a.vec = epilogue_vec(e, out_dtype, 4);
   const size_t stage = static_cast<size_t>(kBoxBytes) * (128 + a.cols / 2);
   a.stages = static_cast<int32_t>(std::min<size_t>(kMaxRing, 216 * 1024 / stage));
-  // all of an SM's shared memory, as all of its tensor memory
-  const size_t smem = std::max<size_t>(a.stages * stage + 1024, 217 * 1024);
   CUtensorMap wm, xm;
   if (!operand_map(&wm, g.w, e.n, g.k, g.swn, g.swk, es, 128) ||
       !operand_map(&xm, g.x, e.m, g.k, g.sxm, g.sxk, es, a.cols / 2))
     return FD_ERR_UNSUPPORTED;
   const int64_t grid = 2 * a.split * (a.split > 1 ? a.mt * a.nt : std::min<int64_t>(pairs, a.mt * a.nt));
-  return from_cuda(launch_cluster(product_pair_kernel<T, FP8>, dim3(static_cast<unsigned>(grid)), kPairThreads,
-                                  2 * a.split, smem, st, wm, xm, a));
+  return from_cuda(launch_cluster<product_pair_kernel<T, FP8>>(dim3(static_cast<unsigned>(grid)), kPairThreads,
+                                                               2 * a.split, kPairSmem, kPairSmem, st, wm, xm, a));
 }
 
 template <typename TX, typename T, bool FP8>
