@@ -70,7 +70,7 @@ FD_DEV uint8_t to_e4m3(float v) { return __nv_cvt_float_to_fp8(v, __NV_SATFINITE
 // again (from L1 or L2) for the maximum and for the values.  Coalesced where the
 // elements are contiguous, so rows that vectors cannot address (odd widths, odd
 // offsets) still stream: SwiGLU of 2100 x 14335 76 us, add_rms_norm_fp8 of 8192 x
-// 4095 109 us.
+// 4095 75 us.
 FD_DEV float block_sum(float v, int warps, float* red) {
   v = warp_sum(v);
   if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
@@ -392,15 +392,19 @@ cudaError_t launch_vec(QuantVecArgs a, bool flat, cudaStream_t st) {
 }
 
 // Threads and register elements for a row of any layout: enough for the row, or
-// the most there are.
+// the most there are; with more rows than SMs fewer threads with more elements,
+// so that several rows share an SM.
 template <typename T, int OP, bool CONTIG>
 cudaError_t launch_generic(const QuantArgs& a, cudaStream_t st) {
-  const dim3 blocks(static_cast<unsigned>(a.rows));
-  using fd_host::launch_pdl;
-  if (a.n <= 1024) return launch_pdl(quant_generic_kernel<T, OP, 128, 8, CONTIG>, blocks, 128, 0, st, a);
-  if (a.n <= 4096) return launch_pdl(quant_generic_kernel<T, OP, 512, 8, CONTIG>, blocks, 512, 0, st, a);
-  if (a.n <= 8192) return launch_pdl(quant_generic_kernel<T, OP, 1024, 8, CONTIG>, blocks, 1024, 0, st, a);
-  return launch_pdl(quant_generic_kernel<T, OP, 1024, 16, CONTIG>, blocks, 1024, 0, st, a);
+  auto go = [&](auto* kernel, int threads) {
+    return fd_host::launch_pdl(kernel, dim3(static_cast<unsigned>(a.rows)), dim3(threads), 0, st, a);
+  };
+  const bool many = a.rows > fd_host::sm_count();
+  if (a.n <= 1024) return go(quant_generic_kernel<T, OP, 128, 8, CONTIG>, 128);
+  if (many && a.n <= 4096) return go(quant_generic_kernel<T, OP, 256, 16, CONTIG>, 256);
+  if (many && a.n <= 8192) return go(quant_generic_kernel<T, OP, 512, 16, CONTIG>, 512);
+  if (a.n <= 8192) return go(quant_generic_kernel<T, OP, 1024, 8, CONTIG>, 1024);
+  return go(quant_generic_kernel<T, OP, 1024, 16, CONTIG>, 1024);
 }
 
 template <int OP>
