@@ -101,7 +101,6 @@ __global__ void __launch_bounds__(128) product_generic_kernel(GenericArgs a) {
   const int wm = (warp & 1) * 32, wn = (warp >> 1) * 32;
   const int64_t n0 = static_cast<int64_t>(blockIdx.x) * kGenTile;
   grid_dep_wait();
-  grid_dep_launch();
   for (int64_t m0 = static_cast<int64_t>(blockIdx.y) * kGenTile; m0 < a.epi.m;
        m0 += static_cast<int64_t>(gridDim.y) * kGenTile) {
     float acc[2][4][4] = {};
@@ -163,6 +162,9 @@ constexpr int kBoxBytes = 128;  // K bytes of a tile row
 constexpr int kMaxRing = 12;
 constexpr int kSliceBytes = 32;  // K bytes of one tcgen05.mma
 
+// None of the product kernels lets the next kernel start before it has finished
+// (grid_dep_launch): y may be the weight of a linear_decode, which streams its
+// weight before it waits.  It costs 0.9 us between products of 4096 x 4096.
 constexpr int kStatusWait = 1;  // a bounded wait expired: the call's output is invalid
 __device__ int g_product_status;
 
@@ -584,7 +586,6 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     __syncwarp();
   }
   grid_dep_wait();
-  grid_dep_launch();
   const int live = static_cast<int>(a.e.m);  // columns in use
   if (warp >= 4) {  // the first tile's part of the epilogue's operands into L2, under its MMAs
     const int et = threadIdx.x - 128;
@@ -631,6 +632,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
           const uint32_t acc = tmem + (static_cast<uint32_t>((warp - 4) * 32) << 16) + b * acc_cols + blk * a.cols;
           for (int c = 0; c < live; c += 16) {
             float v[16], xs[16];
+            __syncwarp();
             tc_load16(acc + c, reinterpret_cast<uint32_t*>(v));
             if (!row_ok) continue;
             if (FP8) {
@@ -657,6 +659,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
         const uint32_t acc = tmem + (static_cast<uint32_t>((warp - 4) * 32) << 16) + blk * a.cols;
         for (int c = 0; c < live; c += 16) {
           uint32_t v[16];
+          __syncwarp();
           tc_load16(acc + c, v);
           if (r < a.rows) {
 #pragma unroll
@@ -787,7 +790,6 @@ __global__ void __launch_bounds__(kPairThreads, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   grid_dep_wait();
-  grid_dep_launch();
 
   if (warp == 0) {
     if (elect_one()) {
@@ -1116,14 +1118,13 @@ int launch_split(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t
   a.tmem_cols = 32;
   while (a.tmem_cols < a.accs * acc) a.tmem_cols *= 2;
   a.vec = epilogue_vec(e, out_dtype, 4);
-  // A ring of half the shared memory lets the next kernel's CTAs start beside
-  // this one's and bring their first tiles into L2; a long stream gains more
-  // from a ring of all of it (28672 x 4096 in 16 bits, 1.6 MB a CTA: 38.9
-  // against 40.1 us; 4096 x 14336 in 8 bits, 0.46 MB a CTA: 14.4 against 14.1).
-  const bool deep = steps / a.split * a.rows * kBoxBytes >= 768 * 1024;
-  a.ahead = deep ? 8 : 4;
+  // A ring of all the shared memory, and the first steps brought into L2 ahead
+  // of the wait: four cost nothing where this kernel starts late, eight delay its
+  // own copies (4096 x 4096 in 8 bits 7.6 against 8.7 us, without any 7.7; the MLP
+  // of one row, behind its row kernels, 39.0 against 39.5 and 41.4).
+  a.ahead = 4;
   const size_t stage = static_cast<size_t>(kBoxBytes) * (a.rows + a.cols);
-  a.stages = static_cast<int32_t>(std::min<size_t>(kMaxRing, (deep ? 216 : 108) * 1024 / stage));
+  a.stages = static_cast<int32_t>(std::min<size_t>(kMaxRing, 216 * 1024 / stage));
   const size_t part = a.split > 1 ? static_cast<size_t>(e.m) * a.rows * 4 : 0;
   // an MMA reads whole blocks of 128 rows, past the last stage's R
   const size_t reads = (a.stages - 1) * stage + static_cast<size_t>(kBoxBytes) * a.blocks * kBlockRows;

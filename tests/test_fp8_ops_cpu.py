@@ -139,3 +139,38 @@ def test_c_entries_refuse_before_any_launch():
 
     assert mlp(p=None) == 3 and mlp(nbytes=need - 1) == 3 and mlp(p=base + 1) == 3
     assert mlp(hidden=None) == bad and mlp(dtype=2) == bad and mlp(i=0) == bad
+
+
+def test_custom_ops_fake_outputs():
+    """Every operator resolves under torch.ops and its fake implementation gives the real one's shapes and types."""
+    ops = torch.ops.fused_decode_b200
+
+    def m(*shape, dtype=BF):
+        return torch.empty(*shape, device="meta", dtype=dtype)
+
+    x = m(2, 3, 64, dtype=F16)
+    for out in (ops.quantize_fp8(x), ops.rms_norm_fp8(x, m(64)), ops.swiglu_fp8(x, x),
+                ops.add_rms_norm_fp8(x, x, m(64))[:2]):
+        assert (out[0].shape, out[0].dtype) == (x.shape, E4M3)
+        assert (out[1].shape, out[1].dtype) == ((2, 3), F32)
+    res = ops.add_rms_norm_fp8(x, x, m(64))[2]
+    assert (res.shape, res.dtype) == (x.shape, F16)
+    y = ops.linear_act(x, m(48, 64, dtype=F16), None, "silu", x)
+    assert (y.shape, y.dtype) == ((2, 3, 48), F16)
+    y = ops.linear_fp8(m(5, 64, dtype=E4M3), m(5, dtype=F32), m(48, 64, dtype=E4M3), m(48, dtype=F32), out_dtype=F16)
+    assert (y.shape, y.dtype) == ((5, 48), F16)
+    h = ops.post_attn_mlp_fp8(m(4, 64), m(64), m(96, 64, dtype=E4M3), m(96, dtype=F32), m(64, 48, dtype=E4M3),
+                              m(64, dtype=F32))
+    assert (h.shape, h.dtype) == ((4, 64), BF)
+
+
+def test_compiled_dispatch_declines_cpu_tensors():
+    fp = _capi.fast()
+    assert fp.quantize_fp8(X, None, None) is None
+    assert fp.rms_norm_fp8(X, W32, 1e-6, None, None) is None
+    assert fp.add_rms_norm_fp8(X, X, W32, 1e-6, None, None, None) is None
+    assert fp.swiglu_fp8(X, X, None, None) is None
+    assert fp.linear_act(X, W, None, None, None, None) is None
+    assert fp.linear_fp8(X8, XS, W8, WS, None, None, None, None, True) is None
+    assert fp.post_attn_mlp_fp8(*MLP, 1e-6) is None
+    assert fp.linear_act("x", None, None, "tanh", None, None) is None

@@ -362,6 +362,36 @@ def test_layer_chain():
     R.check_product(stream, *ref)
 
 
+def test_offsets_beyond_31_bits():
+    """Rows whose elements lie past 2^31: the last ones are right."""
+    g = gen(13)
+    m, n = 66000, 32768
+    x = torch.zeros(m, n, device="cuda", dtype=BF)
+    x[-3:] = rn(g, 3, n)
+    q, s = fd.quantize_fp8(x)
+    R.check_rows8(q[-3:], s[-3:], x[-3:].double())
+    del q, x
+    x, w = rn(g, m, 64), rn(g, n, 64, scale=0.125)
+    y = fd.linear_act(x, w)
+    R.check_product(y[-300:], *R.product(x[-300:], w, None, None, None))
+
+
+def test_product_becomes_the_next_products_weight():
+    """linear_decode streams its weight before it waits for the kernel before
+    it; a product's output is finished by then."""
+    g = gen(14)
+    for rows in (48, 512):
+        a, b, x = rn(g, rows, 2048), rn(g, 2048, 2048, scale=0.02), rn(g, 2, 2048)
+        w = torch.zeros(rows, 2048, device="cuda", dtype=BF)
+        ref_w = fd.linear_act(a, b)
+        torch.cuda.synchronize()
+        ref = fd.linear_decode(x, ref_w)
+        for _ in range(5):
+            w.zero_()
+            fd.linear_act(a, b, out=w)
+            assert torch.equal(fd.linear_decode(x, w), ref)
+
+
 def test_weights_quantised_just_before_use():
     """A product launched behind the kernel that writes its weights waits for it."""
     g = gen(6)
@@ -423,6 +453,48 @@ def test_no_wait_expired():
     from fused_decode_b200 import kernels as K
 
     assert K.product_status() == 0
+
+
+def test_compiled_and_python_paths_agree(monkeypatch):
+    """The compiled dispatch and the Python path behind it give the same bits."""
+    from fused_decode_b200 import ops_fp8
+
+    g = gen(11)
+    x, r, w = rn(g, 3, 4, 256), rn(g, 3, 4, 256), rn(g, 256, dtype=F32)
+    wl, bias = rn(g, 320, 256, scale=0.06), rn(g, 320)
+    res = rn(g, 3, 4, 320)
+    weights = mlp_weights(g, 256, 512)
+
+    def bits(t):
+        return t.view(torch.uint8) if t.dtype == R.E4M3 else t
+
+    def all_calls():
+        q, s = fd.quantize_fp8(x)
+        wq, ws = fd.quantize_fp8(wl)
+        outs = [q, s, *fd.rms_norm_fp8(x, w), *fd.add_rms_norm_fp8(x, r, w), *fd.swiglu_fp8(x, r)]
+        outs += [fd.linear_act(x, wl, bias, activation="gelu", row_add=res), fd.linear_act(x, wl, row_add=bias)]
+        outs += [fd.linear_fp8(q, s, wq, ws, bias, activation="silu", row_add=res)]
+        outs += [fd.linear_fp8(q, s, wq, ws, out_dtype=F16), fd.post_attn_mlp_fp8(x, w, *weights, 1e-5)]
+        return [bits(t) for t in outs]
+
+    assert ops_fp8._fast().linear_act(x, wl, bias, "gelu", res, None) is not None
+    compiled = all_calls()
+    monkeypatch.setattr(ops_fp8, "_fast", lambda: None)
+    python = all_calls()
+    assert all(torch.equal(a, b) for a, b in zip(compiled, python, strict=True))
+
+
+def test_custom_ops():
+    ops = torch.ops.fused_decode_b200
+    g = gen(12)
+    x, w = rn(g, 5, 128), rn(g, 96, 128, scale=0.09)
+    wq, ws = ops.quantize_fp8(w)
+    q, s = ops.rms_norm_fp8(x, torch.ones(128, device="cuda"), 1e-5)
+    assert torch.equal(ops.linear_fp8(q, s, wq, ws, None, "silu", None, F16),
+                       fd.linear_fp8(q, s, wq, ws, activation="silu", out_dtype=F16))
+    assert torch.equal(ops.linear_act(x, w, None, None, None), fd.linear_act(x, w))
+    compiled = torch.compile(lambda t: ops.linear_act(t, w, None, "relu", None), fullgraph=True, backend="eager")
+    assert torch.equal(compiled(x), fd.linear_act(x, w, activation="relu"))
 
 
 def test_cuda_refusals():
