@@ -291,7 +291,7 @@ def linear_act(
     of ``x``'s type or float32; ``row_add`` (a residual) is any 16- or 32-bit
     float tensor that broadcasts to the output.  The sum, the activation and
     both additions are fp32 and the result is rounded once.  ``out`` may be
-    ``row_add`` itself.
+    ``row_add`` itself and may not overlap ``x`` or ``weight``.
     """
     fp = _fast()
     done = fp.linear_act(x, weight, bias, activation, row_add, out) if fp is not None else None
