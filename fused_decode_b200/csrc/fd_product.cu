@@ -392,13 +392,16 @@ FD_DEV void finish4(const Epilogue& e, bool vec, int64_t m, int64_t n, const flo
 // The partial tiles of a cluster's `parts` sharers, `rows` floats to a column
 // at `part` in each: sharer `rank` takes the columns rank, rank + parts, ... below
 // `live`, sums them in sharer order and finishes them, `threads` threads at
-// work.  Sharer p is the cluster's CTA p * step + side.
+// work.  Sharer p is the cluster's CTA p * step + side.  Rows past the last row
+// of w are not read: every remote load then feeds a store to y, so none is still
+// under way when this CTA tells its peers that they may exit.
 template <typename T, bool FP8>
 FD_DEV void join_parts(const Epilogue& e, bool vec, const float* part, int rows, int live, int rank, int parts, int step,
                        int side, int64_t m0, int64_t n0, int tid, int threads) {
   const int quads = rows / 4, mine = live > rank ? (live - rank - 1) / parts + 1 : 0;
   for (int i = tid; i < mine * quads; i += threads) {
     const int c = rank + i / quads * parts, r = i % quads * 4;
+    if (n0 + r >= e.n) continue;
     float4 from[kMaxSplit];  // all on their way before the first is added
 #pragma unroll
     for (int p = 0; p < kMaxSplit; ++p)
@@ -409,7 +412,7 @@ FD_DEV void join_parts(const Epilogue& e, bool vec, const float* part, int rows,
     for (int p = 0; p < kMaxSplit; ++p) {
       v[0] += from[p].x; v[1] += from[p].y; v[2] += from[p].z; v[3] += from[p].w;
     }
-    if (n0 + r < e.n) finish4<T, FP8>(e, vec, m0 + c, n0 + r, v);
+    finish4<T, FP8>(e, vec, m0 + c, n0 + r, v);
   }
 }
 
@@ -677,8 +680,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
                        kSplitThreads);
     __syncwarp();
     // The other CTAs may still be reading this one's partial.  Relaxed, here and
-    // in the pair kernel: nothing is passed on, and a release would wait for
-    // this CTA's stores to y.
+    // in the pair kernel: nothing is passed on, every value read from a peer is in
+    // a store to y that comes before the arrival, and a release would wait for
+    // those stores.
     cluster_arrive_relaxed();
     cluster_wait();
   }

@@ -1,0 +1,51 @@
+"""How the products' kernels split their work on the GPU, against 64-bit forms
+(tests/_fp8_ref.py, which derives the bounds)."""
+
+import pytest
+import torch
+
+from tests import _fp8_ref as R
+
+pytestmark = pytest.mark.gpu
+
+import fused_decode_b200 as fd  # noqa: E402
+
+BF, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def gen(seed=0):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def rn(g, *shape, dtype=BF, scale=1.0):
+    return (torch.randn(*shape, device="cuda", generator=g) * scale).to(dtype)
+
+
+def rows8(g, n, k, scale=1.0):
+    """e4m3 rows with every exponent in use, and scales of their own."""
+    q = (torch.randn(n, k, device="cuda", generator=g) * 40).clamp(-448, 448).to(R.E4M3)
+    return q, (torch.rand(n, device="cuda", generator=g) * 1e-2 + 1e-3) * scale
+
+
+def both_types(seed, m, n, k, act, times=1):
+    """The product in 16 and in 8 bits with bias and row_add: every element, the same bits every time."""
+    g = gen(seed)
+    bias, res = rn(g, n, dtype=F32), rn(g, m, n)
+    x, w = rn(g, m, k), rn(g, n, k, scale=k ** -0.5)
+    y = fd.linear_act(x, w, bias, activation=act, row_add=res)
+    R.check_product(y, *R.product(x, w, bias, act, res))
+    for _ in range(times - 1):
+        assert torch.equal(fd.linear_act(x, w, bias, activation=act, row_add=res), y)
+    (x, xs), (w, ws) = rows8(g, m, k), rows8(g, n, k, k ** -0.5)
+    y = fd.linear_fp8(x, xs, w, ws, bias, activation=act, row_add=res)
+    R.check_product(y, *R.product(x, w, bias, act, res, xs, ws))
+    for _ in range(times - 1):
+        assert torch.equal(fd.linear_fp8(x, xs, w, ws, bias, activation=act, row_add=res), y)
+
+
+# N that leaves most of the last tile without rows of w, K long enough that a
+# cluster shares each tile
+@pytest.mark.parametrize("m,n,k", [(1, 4096, 4096), (2, 8, 8192), (3, 136, 4096), (40, 1000, 4096), (80, 520, 4096),
+                                   (81, 264, 4096), (200, 300, 4096), (640, 520, 4096)])
+def test_shared_tiles_past_the_last_row(m, n, k):
+    both_types(m + n, m, n, k, "silu", times=4)
