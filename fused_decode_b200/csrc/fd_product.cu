@@ -317,6 +317,8 @@ FD_DEV bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort);
 // Wait for the step at `p`, and look at the ring's later stages with the other
 // lanes: how many steps in a row (at most `most`) have arrived, 0 once any role
 // has given up.  One look costs about 150 ns, as much as issuing a step's MMAs.
+// The lane that issues the MMAs has itself looked at one stage only: __syncwarp
+// passes the other lanes' acquires on to it, which the vote alone does not.
 FD_DEV int wait_steps(uint64_t* bars, RingPos p, int stages, int most, volatile int* abort) {
   const int lane = threadIdx.x & 31;
   most = min(most, stages);
@@ -333,6 +335,7 @@ FD_DEV int wait_steps(uint64_t* bars, RingPos p, int stages, int most, volatile 
     if (!wait_or_abort(bars + p.stage, p.phase, abort)) return 0;
     here = 1;
   }
+  __syncwarp();
   return min(here == 0xffffffffu ? 32 : __ffs(~here) - 1, most);
 }
 

@@ -49,3 +49,11 @@ def both_types(seed, m, n, k, act, times=1):
                                    (81, 264, 4096), (200, 300, 4096), (640, 520, 4096)])
 def test_shared_tiles_past_the_last_row(m, n, k):
     both_types(m + n, m, n, k, "silu", times=4)
+
+
+@pytest.mark.parametrize("m,n,k", [(8, 4096, 16384), (64, 9472, 8192), (512, 1024, 16384), (1024, 4096, 8192)])
+def test_long_inner_widths(m, n, k):
+    """Many steps to a tile, so that the MMAs follow the copies through every
+    stage of the ring many times over: whatever landed between two looks, the
+    same bits."""
+    both_types(m, m, n, k, None, times=8)
