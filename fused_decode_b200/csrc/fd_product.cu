@@ -281,8 +281,10 @@ FD_DEV float4 ld_cluster_f4(uint32_t addr) {
   return v;
 }
 
-// Wait (bounded) for the phase of `bar` with this parity.  The bound is looked
-// at every 256 tries.  Acquiring at CTA scope is enough where the other CTA of
+// Wait (bounded) for the phase of `bar` with this parity.  Every role calls
+// grid_dep_wait before its first such wait, so the bound covers this kernel's own
+// work alone, however long the kernels ahead take.  It is looked at every 256
+// tries.  Acquiring at CTA scope is enough where the other CTA of
 // a pair signals, too: what these barriers pass on is shared-memory tiles
 // written by TMA and accumulators in tensor memory, never plain stores.
 constexpr int64_t kWaitClocks = 4000000000ll;  // 2 s at the highest clock
@@ -556,6 +558,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1)
     __syncwarp();
   } else if (warp == 2) {
     const uint64_t ring_desc = tile_desc(smem_addr(ring));  // addresses in 16-byte units: below 2^14
+    // No operand arrives before the kernels ahead have finished: only from there
+    // on does a wait's bound say anything.
+    grid_dep_wait();
     RingPos p{0, 0};
     bool ok = true;
     int it = 0;

@@ -57,3 +57,32 @@ def test_long_inner_widths(m, n, k):
     stage of the ring many times over: whatever landed between two looks, the
     same bits."""
     both_types(m, m, n, k, None, times=8)
+
+
+# One block that lets the next kernel on the stream start at once and then takes
+# 5e9 cycles (2.5 s at 1.97 GHz, 5 s at 1 GHz: more than a bounded wait's 4e9).
+LONG_KERNEL = r"""
+extern "C" __global__ void long_kernel() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const long long t0 = clock64();
+  while (clock64() - t0 < 5000000000ll) __nanosleep(1000);
+}
+"""
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 4096, 1024), (300, 512, 1024)])
+def test_a_long_kernel_ahead_expires_no_wait(m, n, k):
+    """A product that starts early behind a kernel of seconds waits for it
+    without counting that time against its own bound."""
+    from fused_decode_b200 import kernels as K
+
+    g = gen(m)
+    (x, xs), (w, ws) = rows8(g, m, k), rows8(g, n, k, k ** -0.5)
+    ref = fd.linear_fp8(x, xs, w, ws)
+    y = torch.zeros_like(ref)
+    long_kernel = torch.cuda._compile_kernel(LONG_KERNEL, "long_kernel", compute_capability="100")
+    torch.cuda.synchronize()
+    long_kernel(grid=(1, 1, 1), block=(1, 1, 1))
+    fd.linear_fp8(x, xs, w, ws, out=y)
+    assert torch.equal(y, ref)
+    assert K.product_status() == 0
