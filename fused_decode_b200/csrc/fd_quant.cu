@@ -28,6 +28,12 @@ constexpr float kAmaxFloor = 5.421010862427522e-20f;  // 2^-64
 // What a row is before its quantisation.
 enum RowOp { ROW_PLAIN = 0, ROW_RMS = 1, ROW_ADD_RMS = 2, ROW_SWIGLU = 3 };
 
+// Whether the next kernel on the stream may start before this one has finished.
+// Not behind residual_out: a 16-bit tensor may be the weight of a linear_decode,
+// which streams its weight before it waits.
+template <int OP>
+constexpr bool kEarlyNext = OP != ROW_ADD_RMS;
+
 struct QuantArgs {
   RowsArg x;   // plain, norms: the input; SwiGLU: gate
   RowsArg r;   // add+RMSNorm: residual; SwiGLU: up
@@ -95,7 +101,7 @@ __global__ void __launch_bounds__(THREADS) quant_generic_kernel(QuantArgs a) {
   constexpr int warps = THREADS / 32;
   const int64_t row = blockIdx.x;
   grid_dep_wait();
-  grid_dep_launch();
+  if (kEarlyNext<OP>) grid_dep_launch();
   constexpr bool kNorm = OP == ROW_RMS || OP == ROW_ADD_RMS;
   constexpr bool kTwo = OP == ROW_ADD_RMS || OP == ROW_SWIGLU;
   const T* xr = row_ptr<T>(a.x, row, a.B, a.C);
@@ -298,7 +304,7 @@ __global__ void __launch_bounds__(1024) quant_vec_kernel(QuantVecArgs a) {
   const bool live = row < a.g.rows;
   const RowIdx ri = split_row<FLAT>(live ? row : 0, a.g.B, a.g.C);
   grid_dep_wait();
-  grid_dep_launch();
+  if (kEarlyNext<OP>) grid_dep_launch();
 
   Row v;
   RowStats st{0.f, 0.f};

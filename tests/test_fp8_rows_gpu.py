@@ -1,0 +1,28 @@
+"""The 8-bit row operators between other kernels on the stream."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+import fused_decode_b200 as fd  # noqa: E402
+
+BF, F32 = torch.bfloat16, torch.float32
+
+
+# rows of vectors, rows too long for them, and an input at an odd offset
+@pytest.mark.parametrize("rows,n,offset", [(2048, 4096, 0), (8192, 2048, 0), (600, 33000, 0), (4096, 1024, 1)])
+def test_residual_out_becomes_the_next_products_weight(rows, n, offset):
+    """linear_decode streams its weight before it waits for the kernel before
+    it; the norm's residual_out is finished by then, to its last rows."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, res, y = (torch.randn(r, n + offset, device="cuda", generator=g).to(BF)[:, offset:] for r in (rows, rows, 2))
+    nw = torch.ones(n, device="cuda")
+    w = torch.zeros(rows, n, device="cuda", dtype=BF)
+    ref_w = (x.float() + res.float()).to(BF)
+    ref = fd.linear_decode(y, ref_w)
+    for _ in range(20):
+        w.zero_()
+        fd.add_rms_norm_fp8(x, res, nw, 1e-5, residual_out=w)
+        assert torch.equal(fd.linear_decode(y, w), ref)
+        assert torch.equal(w, ref_w)
