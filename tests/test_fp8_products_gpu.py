@@ -86,3 +86,19 @@ def test_a_long_kernel_ahead_expires_no_wait(m, n, k):
     fd.linear_fp8(x, xs, w, ws, out=y)
     assert torch.equal(y, ref)
     assert K.product_status() == 0
+
+
+# Up to 80 rows: N above 256 rows of w for each of the 148 SMs, so that a CTA goes
+# over several tiles -- with two accumulators (up to 64 rows) and with one.
+@pytest.mark.parametrize("m,n,k", [(1, 128256, 1024), (64, 128256, 1024), (65, 128256, 1024), (80, 100003, 640),
+                                   (17, 40000, 2000)])
+def test_several_tiles_to_a_block(m, n, k):
+    both_types(n + m, m, n, k, "relu", times=2)
+
+
+# More rows: at least 149 tiles of 256 by 256 for the 74 pairs of CTAs, both sides
+# ragged, so that each pair goes over three tiles or more with the ring, the
+# accumulators and the scales of x carried from one to the next.
+@pytest.mark.parametrize("m,n,k", [(1990, 5130, 720), (1030, 10313, 528), (300, 40000, 1040), (5000, 2049, 272)])
+def test_several_tiles_to_a_pair(m, n, k):
+    both_types(n + m, m, n, k, "gelu", times=2)

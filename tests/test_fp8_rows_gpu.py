@@ -26,3 +26,18 @@ def test_residual_out_becomes_the_next_products_weight(rows, n, offset):
         fd.add_rms_norm_fp8(x, res, nw, 1e-5, residual_out=w)
         assert torch.equal(fd.linear_decode(y, w), ref)
         assert torch.equal(w, ref_w)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, BF])
+@pytest.mark.parametrize("rows,n", [(1, 1), (40, 4096), (2000, 1024), (9, 77), (300, 5001), (3, 40000)])
+def test_values_and_scales_to_the_bit(rows, n, dtype):
+    """scale = a / 448 and values e4m3(x * (448 / a)), each operation rounded
+    once in fp32: no other value, even where x lies midway between two."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    x = torch.randn(rows, n, device="cuda", generator=g).to(dtype)
+    q, s = fd.quantize_fp8(x)
+    a = x.float().abs().amax(dim=-1).clamp_min(2.0 ** -64)
+    most = torch.full_like(a, 448.0)  # a tensor: torch divides by a number, or a number, through a reciprocal
+    assert torch.equal(s, a / most)
+    want = (x.float() * (most / a)[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
+    assert torch.equal(q.view(torch.uint8), want.view(torch.uint8))
