@@ -630,8 +630,11 @@ def linear_fp8_out(
 
 
 def product_status(device: torch.device | None = None) -> int:
-    """Non-zero once a bounded wait inside a product kernel expired on
-    ``device`` (that call's output is not valid); waits for its current stream."""
+    """Non-zero once a bounded wait inside a product kernel (``linear_act``,
+    ``linear_fp8``, ``post_attn_mlp_fp8``) expired on ``device``: the output of
+    a call since the last ``product_reset`` is not valid.  The calls themselves
+    never wait for the GPU and so cannot raise it.  Waits for the device's
+    current stream; not for use while that stream is captured."""
     import ctypes
 
     word = ctypes.c_int32()
@@ -639,6 +642,13 @@ def product_status(device: torch.device | None = None) -> int:
         status = _capi.load().fd_product_status(word, torch.cuda.current_stream().cuda_stream)
     _capi.check(status, "fd_product_status")
     return word.value
+
+
+def product_reset(device: torch.device | None = None) -> None:
+    """Zero ``product_status``'s word on the device's current stream."""
+    with torch.cuda.device(device):
+        status = _capi.load().fd_product_reset(torch.cuda.current_stream().cuda_stream)
+    _capi.check(status, "fd_product_reset")
 
 
 def post_attn_mlp_fp8_out(

@@ -16,6 +16,10 @@ only, any number of rows, no host synchronisation; like the rest of the
 package the operators launch on the current stream of their tensors' device
 and may be captured in a CUDA graph, and each first offers its arguments to
 the compiled dispatch (``_fastpath``), which takes the common case.
+
+The products' in-kernel waits are bounded (about 2 s).  An expired one leaves
+that call's output invalid without an error: ``kernels.product_status()`` tells
+of it, ``kernels.product_reset()`` clears it.
 """
 
 from __future__ import annotations
