@@ -160,6 +160,11 @@ FD_DEV float silu_mul(float g, float u) {
 // kernel on the stream is still draining.  Every such kernel calls
 // grid_dep_wait() before its first access to global memory another kernel may
 // have written, and grid_dep_launch() once the next kernel may be scheduled.
+// One access comes earlier: the GEMV kernels take their weights for constants and
+// stream them before they wait.  A kernel whose output may be such a weight
+// (add_rms_norm_fp8, the products) leaves grid_dep_launch() out, so that the next
+// kernel starts when its last block is done; the 16-bit row kernels and the GEMVs
+// themselves call it, and what they write is no weight of the launch behind them.
 FD_DEV void grid_dep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 FD_DEV void grid_dep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

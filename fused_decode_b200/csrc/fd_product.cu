@@ -424,8 +424,8 @@ FD_DEV void join_parts(const Epilogue& e, bool vec, const float* part, int rows,
 // N columns of a tile straight from tensor memory, `live` of them in use, one
 // row n of w to a thread: consecutive lanes write consecutive elements of y,
 // whatever its layout.  xs: the scales of the N rows of x.  The columns' offsets
-// from the first are 32-bit (the host keeps 32 row strides of y and row_add
-// below 2^32 elements).
+// from the first are 32-bit (N is 16, and the host keeps row strides of y and
+// row_add below 2^27 elements).
 template <typename T, bool FP8, int N>
 FD_DEV void emit_columns(const Epilogue& e, float* v, int64_t m, int live, int64_t n, const float* xs, float ws,
                          float bias) {
@@ -1095,7 +1095,8 @@ bool epilogue_vec(const Epilogue& e, int out_dtype, int width) {
 // the x tile between two CTAs, wins once x is no longer small beside R.  Split
 // against pair at 64, 80, 96 and 128 rows: 4096 x 4096 in 16 bits 11.8 / 12.8,
 // 12.6 / 13.5, 14.0 / 13.7, 15.1 / 13.8 us; 28672 x 4096 in 8 bits 24.1 / 24.5,
-// 25.4 / 26.0, 26.6 / 25.1, 29.1 / 26.1 us.
+// 25.4 / 26.0, 26.6 / 25.1, 29.1 / 26.1 us.  One number for every N and type: both
+// widths change over between 80 and 96 rows, and others were not measured.
 constexpr int64_t kSplitMaxM = 80;
 
 // Few rows.  FD_ERR_UNSUPPORTED: a layout TMA cannot address.
@@ -1163,8 +1164,9 @@ int launch_pair(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t 
   a.nt = (e.n + kPairRows - 1) / kPairRows;
   // Rows of x per tile and pairs per tile, by the time they should take: a step
   // measured 0.12 us + 0.98 ns per column (0.245 at 128 columns, 0.37 at 256,
-  // MMAs, L2 and the power limit together), a tile's start and end 0.5 us, the
-  // exchange of partials 0.5 us + 6 ns per column.
+  // MMAs, L2 and the power limit together, so for a GPU under steady load; 8 and
+  // 16 bits alike, since a step is 128 bytes of K in either), a tile's start and
+  // end 0.5 us, the exchange of partials 0.5 us + 6 ns per column.
   double best = 0;
   a.cols = 0;
   a.split = 1;
@@ -1206,7 +1208,7 @@ int launch_pair(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t 
 template <typename TX, typename T, bool FP8>
 int launch_product(const GenericArgs& g, int in_dtype, int out_dtype, cudaStream_t st) {
   int r = FD_ERR_UNSUPPORTED;
-  // emit_some's 32-bit column offsets
+  // emit_columns' 32-bit column offsets
   const bool near = g.epi.sym >= 0 && g.epi.srm >= 0 && std::max(g.epi.sym, g.epi.srm) < (int64_t{1} << 27);
   if (g.k > 0 && near) {
     r = g.epi.m <= kSplitMaxM ? launch_split<T, FP8>(g, in_dtype, out_dtype, st)

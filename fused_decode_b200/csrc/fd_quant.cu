@@ -373,8 +373,9 @@ cudaError_t launch_vec2(const QuantVecArgs& a, bool flat, cudaStream_t st) {
 
 // Vectors per thread and warps per row, nv <= 4096.  Many rows run best with four
 // vectors to a thread (add_rms_norm_fp8 8192 x 4096: 42.2 us, with one, two or
-// eight 59, 45, 49), few rows with as many threads a row as a CTA may have (1 x
-// 4096: 2.3 us, with four vectors 3.3).
+// eight 59, 45, 49).  Few rows run best with many threads (1 x 4096: 2.3 us, with
+// four vectors 3.3): one vector each where 16 warps then hold the row, else two,
+// else four as for many rows (8 x 14336: 14 warps, 3.2 us).
 template <typename T, int OP>
 cudaError_t launch_vec(QuantVecArgs a, bool flat, cudaStream_t st) {
   const int nv = a.nv;
