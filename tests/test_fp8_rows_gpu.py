@@ -41,3 +41,26 @@ def test_values_and_scales_to_the_bit(rows, n, dtype):
     assert torch.equal(s, a / most)
     want = (x.float() * (most / a)[:, None]).clamp(-448, 448).to(torch.float8_e4m3fn)
     assert torch.equal(q.view(torch.uint8), want.view(torch.uint8))
+
+
+@pytest.mark.parametrize("rows,n", [(1, 4096), (16, 4096), (148, 8192), (100, 512), (7, 256), (9, 14336), (2, 32768)])
+def test_residual_out_of_few_rows_becomes_the_next_products_weight(rows, n):
+    """As above for few rows, back to back in a graph, without the host's pace between the calls."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, res, y = (torch.randn(r, n, device="cuda", generator=g).to(BF) for r in (rows, rows, 2))
+    nw = torch.ones(n, device="cuda")
+    w = torch.zeros(rows, n, device="cuda", dtype=BF)
+    ref_w = (x.float() + res.float()).to(BF)
+    ref = fd.linear_decode(y, ref_w)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        outs = []
+        for _ in range(20):
+            w.zero_()
+            fd.add_rms_norm_fp8(x, res, nw, 1e-5, residual_out=w)
+            outs.append(fd.linear_decode(y, w))
+    for _ in range(10):
+        graph.replay()
+        for out in outs:
+            assert torch.equal(out, ref)
